@@ -28,6 +28,10 @@ EXPORTS = (
     "hdla_recurrent_fwd", "hdla_chunk_uses_tensor_cores", "hdla_fp32_status_words", "hdla_chunk_fwd_noalloc",
     "hdla_noalloc_read_status", "hdla_recurrent_read_status", "hdla_compose_states", "hdla_param_ab_fwd", "hdla_param_ab_bwd",
     "hdla_norm_gate_fwd", "hdla_norm_gate_bwd",
+    "hdla_short_conv_fwd", "hdla_short_conv_bwd_workspace_bytes", "hdla_short_conv_bwd", "hdla_short_conv_step",
+    "hdla_selective_scan_checkpoint_bytes", "hdla_selective_scan_workspace_bytes", "hdla_selective_scan_fwd",
+    "hdla_selective_scan_bwd", "hdla_selective_scan_step",
+    "hdla_norm_residual_fwd", "hdla_norm_residual_bwd_workspace_bytes", "hdla_norm_residual_bwd",
     # include/hdla_debug.h
     "hdla_kernel_launches", "hdla_timing_enable", "hdla_timing_report", "hdla_debug_tc_buffer",
     "hdla_debug_wait_timeout",

@@ -66,7 +66,7 @@ def binding_built_for(path: str) -> str:
 
 
 def _binding_sources():
-    files = [BINDING_SRC, os.path.join(CSRC, "status_board.h"), os.path.join(ROOT, "include", "hdla.h")]
+    files = [BINDING_SRC, os.path.join(CSRC, "binding_ssm.h"), os.path.join(CSRC, "status_board.h"), os.path.join(ROOT, "include", "hdla.h")]
     return [f for f in files if os.path.exists(f)]
 
 

@@ -50,6 +50,51 @@ static int check_ws(const HdlaDims* d, void* ws, size_t bytes, int with_backward
     return HDLA_OK;
 }
 
+static bool known_type(int dt) { return dt == HDLA_F32 || dt == HDLA_BF16; }
+constexpr int32_t kMaxTokens = 1 << 30;       // token numbers are 32-bit in the kernels, with room for a tile behind the last
+
+static int check_rows(const char* what, int32_t B, int32_t T, int32_t D, int32_t dtype, int32_t n_seqs, const int64_t* cu) {
+    if (B <= 0 || T <= 0 || D <= 0) return fail(HDLA_ERR_INVALID, "%s: non-positive dimension: B=%d T=%d D=%d", what, B, T, D);
+    if (T > kMaxTokens) return fail(HDLA_ERR_UNSUPPORTED, "%s: T=%d, at most %d", what, T, kMaxTokens);
+    if (!known_type(dtype)) return fail(HDLA_ERR_UNSUPPORTED, "%s: dtype %d", what, dtype);
+    if (cu ? (B != 1 || n_seqs < 1) : n_seqs != 0)
+        return fail(HDLA_ERR_INVALID, "%s: n_seqs=%d with B=%d and cu_seqlens %s", what, n_seqs, B, cu ? "given" : "null");
+    return HDLA_OK;
+}
+static int check_conv(const HdlaConvArgs* a) {
+    if (!a) return fail(HDLA_ERR_INVALID, "short_conv: args is null");
+    if (int rc = check_rows("short_conv", a->B, a->T, a->D, a->dtype, a->n_seqs, a->cu_seqlens)) return rc;
+    if (!known_type(a->w_dtype)) return fail(HDLA_ERR_UNSUPPORTED, "short_conv: weight dtype %d", a->w_dtype);
+    if (a->W < 1 || a->W > 8) return fail(HDLA_ERR_UNSUPPORTED, "short_conv: W=%d, 1 to 8 taps are supported", a->W);
+    if (a->activation != HDLA_ACT_NONE && a->activation != HDLA_ACT_SILU)
+        return fail(HDLA_ERR_UNSUPPORTED, "short_conv: activation %d", a->activation);
+    return HDLA_OK;
+}
+static int check_scan(const HdlaScanArgs* a) {
+    if (!a) return fail(HDLA_ERR_INVALID, "selective_scan: args is null");
+    if (int rc = check_rows("selective_scan", a->B, a->T, a->D, a->dtype, a->n_seqs, a->cu_seqlens)) return rc;
+    if (a->N < 1 || a->N > 128) return fail(HDLA_ERR_UNSUPPORTED, "selective_scan: N=%d, 1 to 128 states are supported", a->N);
+    if (a->G < 1 || a->D % a->G) return fail(HDLA_ERR_INVALID, "selective_scan: G=%d groups do not divide D=%d channels", a->G, a->D);
+    return HDLA_OK;
+}
+static int check_norm(const HdlaNormResidualArgs* a) {
+    if (!a) return fail(HDLA_ERR_INVALID, "norm_residual: args is null");
+    if (a->rows <= 0 || a->D <= 0 || a->reserved_ != 0) return fail(HDLA_ERR_INVALID, "norm_residual: bad size");
+    if (a->D > norm_residual_max_d())
+        return fail(HDLA_ERR_UNSUPPORTED, "norm_residual: D=%d, at most %d", a->D, norm_residual_max_d());
+    if (!known_type(a->dtype) || !known_type(a->w_dtype) || (a->r_dtype != a->dtype && a->r_dtype != HDLA_F32))
+        return fail(HDLA_ERR_UNSUPPORTED, "norm_residual: dtype %d, residual %d, weights %d", a->dtype, a->r_dtype, a->w_dtype);
+    if (a->activation < HDLA_ACT_NONE || a->activation > HDLA_ACT_SIGMOID)
+        return fail(HDLA_ERR_UNSUPPORTED, "norm_residual: activation %d", a->activation);
+    return HDLA_OK;
+}
+static int check_space(const char* what, size_t need, const void* ws, size_t bytes) {
+    if (need == 0) return HDLA_OK;
+    if (!ws || reinterpret_cast<uintptr_t>(ws) % 256) return fail(HDLA_ERR_WORKSPACE, "%s: workspace null or not 256-byte aligned", what);
+    if (bytes < need) return fail(HDLA_ERR_WORKSPACE, "%s: workspace too small: %zu < %zu bytes", what, bytes, need);
+    return HDLA_OK;
+}
+
 }  // namespace hdla
 
 using namespace hdla;
@@ -221,6 +266,89 @@ int hdla_norm_gate_bwd(const void* x, const void* gate, const void* weight, cons
     begin_call(static_cast<cudaStream_t>(cuda_stream));
     return norm_gate_launch(true, x, gate, weight, d_o, nullptr, dx, dgate, dweight, rows, D, eps, dtype,
                             static_cast<cudaStream_t>(cuda_stream));
+}
+
+int hdla_short_conv_fwd(const HdlaConvArgs* args, void* cuda_stream) {
+    if (int rc = check_conv(args)) return rc;
+    if (!args->x || !args->weight || !args->y) return fail(HDLA_ERR_INVALID, "short_conv_fwd: null tensor pointer");
+    begin_call(static_cast<cudaStream_t>(cuda_stream));
+    return short_conv_fwd(*args, false, static_cast<cudaStream_t>(cuda_stream));
+}
+
+size_t hdla_short_conv_bwd_workspace_bytes(const HdlaConvArgs* args) {
+    return check_conv(args) == HDLA_OK ? short_conv_bwd_workspace(*args) : 0;
+}
+
+int hdla_short_conv_bwd(const HdlaConvArgs* args, void* workspace, size_t workspace_bytes, void* cuda_stream) {
+    if (int rc = check_conv(args)) return rc;
+    if (!args->x || !args->weight || !args->dx || !args->dweight) return fail(HDLA_ERR_INVALID, "short_conv_bwd: null tensor pointer");
+    if (int rc = check_space("short_conv_bwd", short_conv_bwd_workspace(*args), workspace, workspace_bytes)) return rc;
+    begin_call(static_cast<cudaStream_t>(cuda_stream));
+    return short_conv_bwd(*args, static_cast<float*>(workspace), static_cast<cudaStream_t>(cuda_stream));
+}
+
+int hdla_short_conv_step(const HdlaConvArgs* args, void* cuda_stream) {
+    if (int rc = check_conv(args)) return rc;
+    if (args->T != 1 || args->cu_seqlens) return fail(HDLA_ERR_INVALID, "short_conv_step: one token a sequence, T=%d", args->T);
+    if (!args->x || !args->weight || !args->y || (args->W > 1 && (!args->h0 || args->ht != args->h0)))
+        return fail(HDLA_ERR_INVALID, "short_conv_step: null tensor pointer, or ht is not h0");
+    begin_call(static_cast<cudaStream_t>(cuda_stream));
+    return short_conv_fwd(*args, true, static_cast<cudaStream_t>(cuda_stream));
+}
+
+size_t hdla_selective_scan_checkpoint_bytes(const HdlaScanArgs* args) {
+    return check_scan(args) == HDLA_OK ? selective_scan_checkpoint_bytes(*args) : 0;
+}
+
+size_t hdla_selective_scan_workspace_bytes(const HdlaScanArgs* args, int backward) {
+    return check_scan(args) == HDLA_OK ? selective_scan_workspace(*args, backward != 0) : 0;
+}
+
+int hdla_selective_scan_fwd(const HdlaScanArgs* args, void* workspace, size_t workspace_bytes, void* cuda_stream) {
+    if (int rc = check_scan(args)) return rc;
+    if (!args->x || !args->dt || !args->A || !args->Bm || !args->Cm || !args->y)
+        return fail(HDLA_ERR_INVALID, "selective_scan_fwd: null tensor pointer");
+    if (int rc = check_space("selective_scan_fwd", selective_scan_workspace(*args, false), workspace, workspace_bytes)) return rc;
+    begin_call(static_cast<cudaStream_t>(cuda_stream));
+    return selective_scan_fwd(*args, static_cast<unsigned char*>(workspace), static_cast<cudaStream_t>(cuda_stream));
+}
+
+int hdla_selective_scan_bwd(const HdlaScanArgs* args, void* workspace, size_t workspace_bytes, void* cuda_stream) {
+    if (int rc = check_scan(args)) return rc;
+    if (!args->x || !args->dt || !args->A || !args->Bm || !args->Cm || !args->checkpoints || !args->dx || !args->ddt ||
+        !args->dB || !args->dC || !args->dA || (args->z && !args->dz))
+        return fail(HDLA_ERR_INVALID, "selective_scan_bwd: null tensor pointer");
+    if (int rc = check_space("selective_scan_bwd", selective_scan_workspace(*args, true), workspace, workspace_bytes)) return rc;
+    begin_call(static_cast<cudaStream_t>(cuda_stream));
+    return selective_scan_bwd(*args, static_cast<unsigned char*>(workspace), static_cast<cudaStream_t>(cuda_stream));
+}
+
+int hdla_selective_scan_step(const HdlaScanArgs* args, void* cuda_stream) {
+    if (int rc = check_scan(args)) return rc;
+    if (args->T != 1 || args->cu_seqlens) return fail(HDLA_ERR_INVALID, "selective_scan_step: one token a sequence, T=%d", args->T);
+    if (!args->x || !args->dt || !args->A || !args->Bm || !args->Cm || !args->y || !args->h0 || args->ht != args->h0)
+        return fail(HDLA_ERR_INVALID, "selective_scan_step: null tensor pointer, or ht is not h0");
+    begin_call(static_cast<cudaStream_t>(cuda_stream));
+    return selective_scan_step(*args, static_cast<cudaStream_t>(cuda_stream));
+}
+
+int hdla_norm_residual_fwd(const HdlaNormResidualArgs* args, void* cuda_stream) {
+    if (int rc = check_norm(args)) return rc;
+    if (!args->x || !args->r || (args->pre_weight && !args->u)) return fail(HDLA_ERR_INVALID, "norm_residual_fwd: null tensor pointer");
+    begin_call(static_cast<cudaStream_t>(cuda_stream));
+    return norm_residual_fwd(*args, static_cast<cudaStream_t>(cuda_stream));
+}
+
+size_t hdla_norm_residual_bwd_workspace_bytes(const HdlaNormResidualArgs* args) {
+    return check_norm(args) == HDLA_OK ? norm_residual_bwd_workspace(*args) : 0;
+}
+
+int hdla_norm_residual_bwd(const HdlaNormResidualArgs* args, void* workspace, size_t workspace_bytes, void* cuda_stream) {
+    if (int rc = check_norm(args)) return rc;
+    if (!args->x || !args->dx) return fail(HDLA_ERR_INVALID, "norm_residual_bwd: null tensor pointer");
+    if (int rc = check_space("norm_residual_bwd", norm_residual_bwd_workspace(*args), workspace, workspace_bytes)) return rc;
+    begin_call(static_cast<cudaStream_t>(cuda_stream));
+    return norm_residual_bwd(*args, static_cast<float*>(workspace), static_cast<cudaStream_t>(cuda_stream));
 }
 
 }  // extern "C"

@@ -771,6 +771,10 @@ PyObject* py_set_decay(PyObject*, PyObject* const* av, Py_ssize_t n) {
     Py_RETURN_NONE;
 }
 
+}  // namespace
+#include "binding_ssm.h"
+namespace {
+
 // bind(handle of the loaded libhdla, callable that warns of the fp32 rerun)
 PyObject* py_bind(PyObject*, PyObject* const* av, Py_ssize_t n) {
     if (n != 2) { PyErr_SetString(PyExc_TypeError, "bind(handle, on_overflow)"); return nullptr; }
@@ -790,6 +794,7 @@ PyObject* py_bind(PyObject*, PyObject* const* av, Py_ssize_t n) {
             look_up(h, "hdla_norm_gate_bwd", abi.norm_gate_bwd);
             look_up(h, "hdla_last_error", abi.last_error);
             look_up(h, "hdla_recurrent_fwd", abi.recurrent_fwd);
+            bind_ssm(h);
             look_up(h, "hdla_chunk_fwd", abi.chunk_fwd);
         }))
         return nullptr;
@@ -808,6 +813,14 @@ PyMethodDef methods[] = {{"bind", FAST(py_bind), nullptr},
                          {"chunk_backward", FAST(py_chunk_backward), nullptr},
                          {"recurrent", FAST(py_recurrent), nullptr},
                          {"norm_gate", FAST(py_norm_gate), nullptr},
+                         {"short_conv", FAST(py_short_conv), nullptr},
+                         {"short_conv_backward", FAST(py_short_conv_backward), nullptr},
+                         {"short_conv_step", FAST(py_short_conv_step), nullptr},
+                         {"selective_scan", FAST(py_selective_scan), nullptr},
+                         {"selective_scan_backward", FAST(py_selective_scan_backward), nullptr},
+                         {"selective_scan_step", FAST(py_selective_scan_step), nullptr},
+                         {"norm_residual", FAST(py_norm_residual), nullptr},
+                         {"norm_residual_backward", FAST(py_norm_residual_backward), nullptr},
                          {"status_check", FAST(py_status_check), nullptr},
                          {"status_post", py_status_post, METH_O, nullptr},
                          {"decay", py_decay, METH_O, nullptr},

@@ -129,6 +129,20 @@ constexpr float kNormEps = 1e-5f;
 int norm_gate_launch(bool backward, const void* x, const void* gate, const void* weight, const void* d_o, void* o,
                      void* dx, void* dgate, float* dweight, long long rows, int D, float eps, int dt, cudaStream_t st);
 
+// selective state space mixer: short_conv.cu, selective_scan.cu, norm_residual.cu
+int short_conv_fwd(const HdlaConvArgs& a, bool step, cudaStream_t st);
+size_t short_conv_bwd_workspace(const HdlaConvArgs& a);
+int short_conv_bwd(const HdlaConvArgs& a, float* part, cudaStream_t st);
+size_t selective_scan_checkpoint_bytes(const HdlaScanArgs& a);
+size_t selective_scan_workspace(const HdlaScanArgs& a, bool backward);
+int selective_scan_fwd(const HdlaScanArgs& a, unsigned char* ws, cudaStream_t st);
+int selective_scan_bwd(const HdlaScanArgs& a, unsigned char* ws, cudaStream_t st);
+int selective_scan_step(const HdlaScanArgs& a, cudaStream_t st);
+int norm_residual_max_d();
+int norm_residual_fwd(const HdlaNormResidualArgs& a, cudaStream_t st);
+size_t norm_residual_bwd_workspace(const HdlaNormResidualArgs& a);
+int norm_residual_bwd(const HdlaNormResidualArgs& a, float* part, cudaStream_t st);
+
 // tensor-core (bf16) pipeline, chunk_tc.cu
 bool tc_supported(const HdlaDims& d);
 size_t tc_workspace_bytes(const HdlaDims& d, int with_backward);

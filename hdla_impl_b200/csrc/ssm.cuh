@@ -1,0 +1,237 @@
+// Shared by the short convolution, the selective scan and the norms round a block: packed sequences, groups of channels
+// moved as one access, activations, and sums over partial rows in a fixed order.
+#pragma once
+#include "common.cuh"
+
+namespace hdla {
+namespace {
+
+// ------------------------------------------------------------------------------------------ sequences
+// The sequences along one row of T tokens: the whole row, or those of a packed batch.  Offsets are cut to 0..T where they
+// are read, so that no offset makes a kernel leave its tensors.
+struct Seqs {
+    const int64_t* cu;
+    int n, T;
+    __device__ __forceinline__ int off(int i) const {
+        if (i == 0) return 0;
+        if (!cu) return T;
+        const long long c = __ldg(reinterpret_cast<const long long*>(cu) + i);
+        return static_cast<int>(c < 0 ? 0 : c > T ? T : c);
+    }
+    __device__ __forceinline__ int end() const { return off(n); }          // rows from here on belong to no sequence
+    // the first sequence that ends behind token t, or n
+    __device__ __forceinline__ int ends_behind(int t) const {
+        int lo = 0, hi = n;
+        while (lo < hi) {
+            const int m = (lo + hi) >> 1;
+            if (off(m + 1) > t) hi = m; else lo = m + 1;
+        }
+        return lo;
+    }
+    // the last sequence that starts before token t (t > 0)
+    __device__ __forceinline__ int starts_before(int t) const {
+        int lo = 0, hi = n - 1;
+        while (lo < hi) {
+            const int m = (lo + hi + 1) >> 1;
+            if (off(m) < t) lo = m; else hi = m - 1;
+        }
+        return lo;
+    }
+};
+
+// ------------------------------------------------------------------------------------------ channels
+// PW neighbouring channels of a row.  Vec: one access of PW elements (the address is a multiple of its size and all
+// channels exist); otherwise element by element, `valid` of them.
+template <int DT, int PW>
+struct Pack { uint32_t w[PW * (DT == HDLA_F32 ? 4 : 2) / 4]; };
+
+template <int N>
+__device__ __forceinline__ void ld_words(uint32_t* w, const void* p) {
+    if constexpr (N % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            const uint4 v = *reinterpret_cast<const uint4*>(static_cast<const uint32_t*>(p) + i);
+            w[i] = v.x; w[i + 1] = v.y; w[i + 2] = v.z; w[i + 3] = v.w;
+        }
+    } else if constexpr (N == 2) {
+        const uint2 v = *static_cast<const uint2*>(p);
+        w[0] = v.x; w[1] = v.y;
+    } else {
+        w[0] = *static_cast<const uint32_t*>(p);
+    }
+}
+template <int N>
+__device__ __forceinline__ void st_words(void* p, const uint32_t* w) {
+    if constexpr (N % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4)
+            *reinterpret_cast<uint4*>(static_cast<uint32_t*>(p) + i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+    } else if constexpr (N == 2) {
+        *static_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    } else {
+        *static_cast<uint32_t*>(p) = w[0];
+    }
+}
+template <int DT>
+__device__ __forceinline__ const char* elem_ptr(const void* base, long long i) {
+    return static_cast<const char*>(base) + i * (DT == HDLA_F32 ? 4 : 2);
+}
+
+template <int DT, int PW, bool Vec>
+__device__ __forceinline__ Pack<DT, PW> ld_pack(const void* base, long long i, int valid) {
+    Pack<DT, PW> r;
+    constexpr int NW = sizeof(r.w) / 4;
+    if constexpr (Vec) {
+        if (valid > 0) ld_words<NW>(r.w, elem_ptr<DT>(base, i));
+        else
+#pragma unroll
+            for (int j = 0; j < NW; ++j) r.w[j] = 0;
+    } else if constexpr (DT == HDLA_F32) {
+#pragma unroll
+        for (int j = 0; j < PW; ++j) r.w[j] = j < valid ? static_cast<const uint32_t*>(base)[i + j] : 0u;
+    } else {
+#pragma unroll
+        for (int j = 0; j < NW; ++j) {
+            const uint32_t lo = 2 * j < valid ? static_cast<const uint16_t*>(base)[i + 2 * j] : 0u;
+            const uint32_t hi = 2 * j + 1 < valid ? static_cast<const uint16_t*>(base)[i + 2 * j + 1] : 0u;
+            r.w[j] = lo | hi << 16;
+        }
+    }
+    return r;
+}
+template <int DT, int PW>
+__device__ __forceinline__ void unpack(const Pack<DT, PW>& r, float* f) {
+    if constexpr (DT == HDLA_F32) {
+#pragma unroll
+        for (int j = 0; j < PW; ++j) f[j] = __uint_as_float(r.w[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < PW / 2; ++j) {
+            f[2 * j] = __uint_as_float(r.w[j] << 16);
+            f[2 * j + 1] = __uint_as_float(r.w[j] & 0xffff0000u);
+        }
+    }
+}
+// The one rounding of an output to its type.
+template <int DT, int PW, bool Vec>
+__device__ __forceinline__ void st_pack(void* base, long long i, int valid, const float* f) {
+    if constexpr (Vec) {
+        if (valid <= 0) return;
+        Pack<DT, PW> r;
+        if constexpr (DT == HDLA_F32) {
+#pragma unroll
+            for (int j = 0; j < PW; ++j) r.w[j] = __float_as_uint(f[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < PW / 2; ++j) {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * j], f[2 * j + 1]);
+                r.w[j] = *reinterpret_cast<const uint32_t*>(&h);
+            }
+        }
+        st_words<sizeof(r.w) / 4>(const_cast<char*>(elem_ptr<DT>(base, i)), r.w);
+    } else {
+#pragma unroll
+        for (int j = 0; j < PW; ++j)
+            if (j < valid) st_elem(base, i + j, DT, f[j]);
+    }
+}
+
+// ------------------------------------------------------------------------------------------ activations
+__device__ __forceinline__ float sigmoid_of(float v) { return __fdividef(1.f, 1.f + __expf(-v)); }   // (e^-v = inf: 0)
+__device__ __forceinline__ float act_of(float v, int act) {
+    return act == HDLA_ACT_SILU ? v * sigmoid_of(v) : act == HDLA_ACT_SIGMOID ? sigmoid_of(v) : v;
+}
+__device__ __forceinline__ float act_grad(float v, int act) {
+    if (act == HDLA_ACT_NONE) return 1.f;
+    const float s = sigmoid_of(v);
+    return act == HDLA_ACT_SILU ? s * (1.f + v * (1.f - s)) : s * (1.f - s);
+}
+// log(1 + e^v) = max(v, 0) + log1p(e), e = e^-|v| in (0, 1]: log1p(e) = 2 artanh(s), s = e / (2 + e) <= 1/3, by the series
+// s + s^3/3 + ... + s^13/13, whose remainder at s = 1/3 is 1.6e-8 of the sum.  (A logarithm of 1 + e would lose the
+// small time steps: they are e itself.)  `e` is handed back for the derivative.
+__device__ __forceinline__ float softplus_of(float v, float& e) {
+    e = __expf(-fabsf(v));
+    const float s = __fdividef(e, 2.f + e), q = s * s;
+    float p = fmaf(q, 1.f / 13.f, 1.f / 11.f);
+    p = fmaf(p, q, 1.f / 9.f);
+    p = fmaf(p, q, 1.f / 7.f);
+    p = fmaf(p, q, 1.f / 5.f);
+    p = fmaf(p, q, 1.f / 3.f);
+    p = fmaf(p, q, 1.f);
+    return fmaxf(v, 0.f) + 2.f * s * p;
+}
+
+// ------------------------------------------------------------------------------------------ sums over partial rows
+// out[c] = sum over P rows of part[row, c], in the rows' order by eight- and sixteenfold strides that depend on P alone.
+// Column c = (r * K + k) * NP + n goes to out[k][r * N + n] where n < N; with `turned` column n * K + k of a [NP, K] matrix
+// (r = 0), as the convolution's taps are laid out.
+struct ColJob {
+    const float* part;
+    void* out[3];
+    long long C;
+    int P, K, NP, N, dt, turned, per_lane;
+    unsigned first_block;
+};
+struct ColJobs { ColJob j[3]; int n; };
+constexpr int kColRows = 16;
+
+__device__ __forceinline__ void col_store(const ColJob& j, long long c, float v) {
+    const long long rk = c / j.NP;
+    const int n = static_cast<int>(c - rk * j.NP), k = static_cast<int>(rk % j.K);
+    if (n >= j.N) return;
+    if (j.turned) {                                   // rows 0..K-2 are the taps, row K-1 the bias
+        if (k < j.K - 1) st_elem(j.out[0], (size_t)n * (j.K - 1) + k, j.dt, v);
+        else if (j.out[1]) st_elem(j.out[1], n, j.dt, v);
+        return;
+    }
+    void* out = k == 0 ? j.out[0] : k == 1 ? j.out[1] : j.out[2];
+    if (out) st_elem(out, (rk / j.K) * j.N + n, j.dt, v);
+}
+
+__global__ void __launch_bounds__(32 * kColRows) column_sum_kernel(ColJobs js) {
+    __shared__ float red[kColRows][4][32];
+    int which = 0;
+    while (which + 1 < js.n && blockIdx.x >= js.j[which + 1].first_block) ++which;
+    const ColJob& j = js.j[which];
+    const int lane = threadIdx.x & 31, row = threadIdx.x >> 5;
+    const long long c0 = (long long)(blockIdx.x - j.first_block) * 32 * j.per_lane + lane;
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int p = row; p < j.P; p += kColRows) {
+        const float* at = j.part + (long long)p * j.C;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i < j.per_lane && c0 + 32 * i < j.C) s[i] += at[c0 + 32 * i];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) red[row][i][lane] = s[i];
+    __syncthreads();
+    if (row < j.per_lane) {
+        float t = 0.f;
+#pragma unroll
+        for (int r = 0; r < kColRows; ++r) t += red[r][row][lane];
+        const long long c = c0 + 32 * row;
+        if (c < j.C) col_store(j, c, t);
+    }
+}
+
+// Wide jobs (enough columns to fill the GPU at four a lane) take four a lane: fewer blocks, more loads in flight each.
+inline int column_sum_launch(ColJobs& js, cudaStream_t st) {
+    long long at = 0;
+    for (int i = 0; i < js.n; ++i) {
+        ColJob& j = js.j[i];
+        j.first_block = static_cast<unsigned>(at);
+        j.per_lane = j.C >= 128LL * 4 * sm_count() ? 4 : 1;
+        at += (j.C + 32 * j.per_lane - 1) / (32 * j.per_lane);
+    }
+    if (at > 0x7fffffffLL) return fail(HDLA_ERR_UNSUPPORTED, "column sums: %lld blocks", at);
+    column_sum_kernel<<<static_cast<unsigned>(at), 32 * kColRows, 0, st>>>(js);
+    HDLA_CHECK_LAUNCH("column_sum_kernel");
+    return HDLA_OK;
+}
+
+inline bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+inline size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+
+}  // namespace
+}  // namespace hdla

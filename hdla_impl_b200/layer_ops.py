@@ -12,6 +12,9 @@ written or read and the operator's input is 4 tensors of ``[B,T,H,K]`` plus beta
 ``rms_norm_fused_gate`` -- the layer's output epilogue, RMS norm of ``x * sigmoid(gate)`` over the hidden
 row times a weight (reference: RMSNormFusedGate, HRDPLR/normalizations/rms_norm.py:48-91 with
 gate_act="sigmoid", gate_pos="pre"), forward and backward kernels ``hdla_norm_gate_fwd`` / ``_bwd``.
+
+``rms_norm_residual`` -- what stands between two blocks, as one call: the RMS norm after a block, its gate, the residual scale
+and sum, and the RMS norm before the next block (``hdla_norm_residual_fwd`` / ``_bwd``; no counterpart in the reference).
 """
 from __future__ import annotations
 
@@ -213,3 +216,72 @@ def rms_norm_fused_gate(x: torch.Tensor, gate: torch.Tensor, weight: torch.Tenso
     """``sqrt(D) * y / sqrt(sum(y^2) + eps) * weight`` with ``y = x * sigmoid(gate)`` over the last dimension."""
     r = (_lib._native or _lib.native()).norm_gate(x, gate, weight, eps)
     return _NormGate.apply(x, gate, weight, eps) if r is NotImplemented else r
+
+
+class _NormResidual(torch.autograd.Function):
+    """The operator for arguments that need a Python autograd function (tensor subclasses, tracing)."""
+
+    @staticmethod
+    @_op.autocast_custom_fwd
+    def forward(ctx, x, residual, gate, scale, post_weight, pre_weight, act, eps):
+        ctx.scale = None if torch.is_tensor(scale) else scale
+        ctx.act, ctx.eps = act, eps
+        ctx.save_for_backward(x, residual, gate, scale if ctx.scale is None else None, post_weight, pre_weight)
+        r = _lib.native().norm_residual(*_NormResidual._args(ctx, (x, residual, gate, scale, post_weight, pre_weight)))
+        if r is NotImplemented:
+            raise TypeError("rms_norm_residual: unsupported arguments")
+        return r
+
+    @staticmethod
+    def _args(ctx, t):
+        x, residual, gate, scale, post, pre = [_op._plain(v) if torch.is_tensor(v) else v for v in t]
+        return x, residual, gate, scale if ctx.scale is None else ctx.scale, post, pre, ctx.act, ctx.eps
+
+    @staticmethod
+    @_op.autocast_custom_bwd
+    def backward(ctx, dr, du):
+        g = _lib.native().norm_residual_backward(*_NormResidual._args(ctx, ctx.saved_tensors), _op._plain(dr), _op._plain(du))
+        return (*g, None, None)
+
+
+_GATE_ACTS = {None: 0, "silu": 1, "sigmoid": 2}
+
+
+@torch.compiler.disable
+def rms_norm_residual(
+    x: torch.Tensor,                                # [..., D]  a block's output
+    residual: Optional[torch.Tensor] = None,        # [..., D]  of x's type, or fp32
+    *,
+    gate: Optional[torch.Tensor] = None,            # [..., D]
+    scale=1.0,                                      # a number, or [D]
+    post_weight: Optional[torch.Tensor] = None,     # [D]  weight of the norm after the block; None: no norm
+    pre_weight: Optional[torch.Tensor] = None,      # [D]  weight of the norm before the next block; None: no norm
+    gate_act: Optional[str] = "sigmoid",            # "sigmoid", "silu" or None
+    eps: float = 1e-5,
+) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """``v = rms(x) * post_weight``, ``v = v * act(gate)``, ``r = residual + scale * v``, ``u = rms(r) * pre_weight`` with
+    ``rms(a) = sqrt(D) a / sqrt(sum(a^2) + eps)``; returns ``(r, u)``, u None without ``pre_weight``.  Each part whose tensor is
+    None is left out.  Rows of up to 8192 channels; r has the residual's type, u has x's; u is formed from r before its rounding."""
+    if gate_act not in _GATE_ACTS:
+        raise ValueError(f"gate_act {gate_act!r} must be 'sigmoid', 'silu' or None")
+    act = _GATE_ACTS[gate_act]
+    out = (_lib._native or _lib.native()).norm_residual(x, residual, gate, scale, post_weight, pre_weight, act, eps)
+    if out is not NotImplemented:
+        return out
+    vectors = {"post_weight": post_weight, "pre_weight": pre_weight, "scale": scale if torch.is_tensor(scale) else None}
+    _lib.require_cuda(x, residual, gate, *vectors.values())
+    if x.dim() < 1 or x.numel() == 0 or x.shape[-1] > 8192:
+        raise ValueError(f"x {tuple(x.shape)} must hold rows of 1 to 8192 channels")
+    for name, t in (("residual", residual), ("gate", gate)):
+        if t is not None and t.shape != x.shape:
+            raise ValueError(f"{name} {tuple(t.shape)} must be shaped like x {tuple(x.shape)}")
+    _lib.dtype_code(x.dtype)
+    if gate is not None and gate.dtype != x.dtype:
+        raise TypeError(f"gate must be {x.dtype} like x, not {gate.dtype}")
+    if residual is not None and residual.dtype not in (x.dtype, torch.float32):
+        raise TypeError(f"residual must be {x.dtype} like x, or float32, not {residual.dtype}")
+    for name, t in vectors.items():
+        if t is not None and (tuple(t.shape) != (x.shape[-1],) or not t.is_floating_point()):
+            raise ValueError(f"{name} must be a floating-point vector [D] with D={x.shape[-1]}")
+    return _NormResidual.apply(x, residual, gate, scale if torch.is_tensor(scale) else float(scale), post_weight, pre_weight, act,
+                               float(eps))

@@ -27,7 +27,7 @@
 extern "C" {
 #endif
 
-#define HDLA_VERSION 103
+#define HDLA_VERSION 104
 
 #if defined(__GNUC__)
 #define HDLA_API __attribute__((visibility("default")))
@@ -270,6 +270,103 @@ HDLA_API int hdla_norm_gate_fwd(const void* x, const void* gate, const void* wei
 HDLA_API int hdla_norm_gate_bwd(const void* x, const void* gate, const void* weight, const void* d_o,
                                 void* dx, void* dgate, float* dweight,
                                 int64_t rows, int32_t D, float eps, int32_t dtype, void* cuda_stream);
+
+/* ---------------------------------------------------------------------------------------------------------------
+ * Selective state space mixer: short causal convolution, selective scan, and the norms round a block.  No counterparts
+ * in the reference; they are what a model needs that mixes such blocks with the delta rule's.
+ *
+ * Every call takes one argument struct.  Activations share `dtype` (HDLA_F32 or HDLA_BF16); channels lie next to each
+ * other, the strides between sequences (`*_batch`) and tokens (`*_token`) are given in elements where an input may be a
+ * slice of a wider tensor, and outputs, gradients and states are dense.  Any size and any element alignment is taken;
+ * 16-byte aligned tensors whose strides are multiples of 16 bytes run faster.
+ *
+ * Packed batches: with cu_seqlens (DEVICE array of n_seqs + 1 offsets that do not decrease; its first entry counts as
+ * 0) B is 1, sequence s holds tokens [cu_seqlens[s], cu_seqlens[s+1]) and has state s.  Sequences may be empty: their
+ * final state is their initial one.  Rows from cu_seqlens[n_seqs] on belong to no sequence: outputs and gradients there
+ * are zero.  Offsets outside 0..T are cut to that range.
+ * Sums over rows (gradients of weights, of shared B and C) are taken in a fixed order: the same call gives the same bits. */
+#define HDLA_ACT_NONE    0
+#define HDLA_ACT_SILU    1
+#define HDLA_ACT_SIGMOID 2
+
+/* Depthwise causal convolution over W taps (1..8) and its activation (none or silu):
+ *     p_t = bias + sum_{k<W} weight[W-1-k] x_{t-k},   y_t = act(p_t)
+ * Rows before a sequence's first token come from its initial state [n, W-1, D] (row W-2 is the most recent), or are zero. */
+typedef struct HdlaConvArgs {
+    int32_t B, T, D, W;
+    int32_t dtype;               /* x, y, states and their gradients                                  */
+    int32_t w_dtype;             /* weight [D, W], bias [D] and their gradients                       */
+    int32_t activation;          /* HDLA_ACT_NONE | HDLA_ACT_SILU                                     */
+    int32_t n_seqs;              /* of a packed batch, else 0                                         */
+    const int64_t* cu_seqlens;
+    int64_t x_batch, x_token;    /* strides of x                                                      */
+    const void *x, *weight, *bias, *h0;      /* bias, h0 may be null                                  */
+    void *y, *ht;                            /* forward: [B,T,D]; [n, W-1, D] or null                 */
+    const void *dy, *dht;                    /* backward: either may be null (zero)                   */
+    void *dx, *dh0;                          /* dh0 may be null                                       */
+    void *dweight, *dbias;                   /* [D, W], [D], overwritten; dbias may be null           */
+} HdlaConvArgs;
+
+HDLA_API int hdla_short_conv_fwd(const HdlaConvArgs* args, void* cuda_stream);
+HDLA_API size_t hdla_short_conv_bwd_workspace_bytes(const HdlaConvArgs* args);
+HDLA_API int hdla_short_conv_bwd(const HdlaConvArgs* args, void* workspace, size_t workspace_bytes, void* cuda_stream);
+/* One token for each of B sequences (T = 1): y [B, D], and the state ht = h0 [B, W-1, D] moved on in place. */
+HDLA_API int hdla_short_conv_step(const HdlaConvArgs* args, void* cuda_stream);
+
+/* Selective scan over D channels with N states each (1..128); groups of D / G channels share B and C:
+ *     d_t = softplus(dt_t + dt_bias) or dt_t + dt_bias
+ *     h_t[n] = exp(d_t A[n]) h_{t-1}[n] + d_t x_t B_t[n],    y_t = (sum_n C_t[n] h_t[n] + skip x_t) silu(z_t)
+ * A holds decay rates (<= 0).  States are fp32. */
+typedef struct HdlaScanArgs {
+    int32_t B, T, D, N, G;
+    int32_t dtype;               /* x, dt, z, Bm, Cm, y and their gradients                           */
+    int32_t softplus;            /* dt passes through softplus                                        */
+    int32_t n_seqs;              /* of a packed batch, else 0                                         */
+    const int64_t* cu_seqlens;
+    int64_t x_batch, x_token, dt_batch, dt_token, z_batch, z_token;
+    int64_t B_batch, B_token, B_group, C_batch, C_token, C_group;      /* states lie next to each other */
+    const void *x, *dt, *z, *Bm, *Cm;        /* [B,T,D], [B,T,D], [B,T,D] or null, [B,T,G,N] twice     */
+    const float *A, *skip, *dt_bias, *h0;    /* [D,N], [D] or null, [D] or null, [n,D,N] or null      */
+    void* y;
+    float* ht;                               /* [n,D,N] or null                                       */
+    float* checkpoints;                      /* forward writes, backward reads: hdla_selective_scan_checkpoint_bytes;
+                                                null where no backward follows                        */
+    const void* dy;                          /* backward: may be null (zero)                          */
+    const float* dht;                        /* may be null (zero)                                    */
+    void *dx, *ddt, *dz, *dB, *dC;           /* dz may be null without z                              */
+    float *dA, *dskip, *ddt_bias, *dh0;      /* dA [D,N]; dskip, ddt_bias [D], dh0: null where not wanted */
+} HdlaScanArgs;
+
+HDLA_API size_t hdla_selective_scan_checkpoint_bytes(const HdlaScanArgs* args);
+HDLA_API size_t hdla_selective_scan_workspace_bytes(const HdlaScanArgs* args, int backward);      /* forward: may be 0 */
+HDLA_API int hdla_selective_scan_fwd(const HdlaScanArgs* args, void* workspace, size_t workspace_bytes, void* cuda_stream);
+HDLA_API int hdla_selective_scan_bwd(const HdlaScanArgs* args, void* workspace, size_t workspace_bytes, void* cuda_stream);
+/* One token for each of B sequences (T = 1): y [B, D], and the state ht = h0 [B, D, N] moved on in place. */
+HDLA_API int hdla_selective_scan_step(const HdlaScanArgs* args, void* cuda_stream);
+
+/* RMS norms after and before a block, with the block's gate, residual scale and residual sum, per row of D channels:
+ *     v = x  or  rms(x) post_weight;   v = v act(gate);   r = residual + scale v;   u = rms(r) pre_weight
+ * rms(a) = sqrt(D) a / sqrt(sum a^2 + eps), as in hdla_norm_gate_fwd.  `scale` is a vector [D] or null (then the number
+ * `scale_value`). */
+typedef struct HdlaNormResidualArgs {
+    int64_t rows;
+    int32_t D;
+    int32_t dtype;               /* x, gate, u and their gradients                                    */
+    int32_t r_dtype;             /* residual, r and their gradients                                   */
+    int32_t w_dtype;             /* post_weight, pre_weight, scale and their gradients                */
+    int32_t activation;          /* of the gate: HDLA_ACT_NONE | HDLA_ACT_SILU | HDLA_ACT_SIGMOID     */
+    float eps, scale_value;
+    int32_t reserved_;           /* keep 0                                                            */
+    const void *x, *residual, *gate, *post_weight, *pre_weight, *scale;      /* all but x may be null */
+    void *r, *u;                             /* forward: u null without pre_weight                    */
+    const void *dr, *du;                     /* backward: either may be null (zero)                   */
+    void *dx, *dresidual, *dgate;            /* null where the input is                               */
+    void *dpost_weight, *dpre_weight, *dscale;       /* [D], overwritten; null where the input is      */
+} HdlaNormResidualArgs;
+
+HDLA_API int hdla_norm_residual_fwd(const HdlaNormResidualArgs* args, void* cuda_stream);
+HDLA_API size_t hdla_norm_residual_bwd_workspace_bytes(const HdlaNormResidualArgs* args);
+HDLA_API int hdla_norm_residual_bwd(const HdlaNormResidualArgs* args, void* workspace, size_t workspace_bytes, void* cuda_stream);
 
 #ifdef __cplusplus
 }
