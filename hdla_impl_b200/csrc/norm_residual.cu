@@ -2,48 +2,66 @@
 //     v = x or rms(x) post;   v = v act(gate);   r = residual + scale v;   u = rms(r) pre,   rms(a) = sqrt(D) a / sqrt(sum a^2 + eps)
 // forward and backward as one kernel each: every tensor is read or written once, which is what bounds them (HBM).
 //
-// A thread owns eight neighbouring channels of a row (16-byte accesses of bf16) and holds them between the sums; a row takes
-// as many whole warps as it needs, narrow rows share a block.  Blocks walk over rows and request the next row's tensors
-// before the sums of this one.  Backward computes r again from the inputs in fp32 (as many bytes as reading the rounded r),
-// takes three sums (x^2; r^2 with the dot product of the pre norm's gradient; that of the post norm's), and keeps the sums
-// over rows (gradients of the weights and of scale) in registers until its last row; blocks' sums are added in a fixed order.
+// A thread owns eight neighbouring channels of a row (16-byte accesses of bf16) and holds them, as packed pairs, between the
+// sums; a row takes as many whole warps as it needs, narrow rows share a block.  Blocks walk over rows and request the next
+// row's tensors before the sums of this one; the weights wait in shared memory, so that two (backward) or four (forward) blocks
+// of 256 threads fit on an SM: with them in registers backward had one, and took 686 instead of 300 us for 32768 rows of 2048.
+// Backward computes r again from the inputs in fp32 (as many bytes as reading the rounded r), takes three sums (x^2; r^2 with
+// the dot product of the pre norm's gradient; that of the post norm's), and keeps the sums over rows (gradients of the weights
+// and of scale) in registers until its last row; blocks' sums are added in a fixed order.  Rows of more than 4096 channels
+// need 1024 threads of 64 registers: there those sums are in shared memory too, and nothing is requested ahead.
+#include "f32x2.cuh"
 #include "ssm.cuh"
 
 namespace hdla {
 namespace {
 
-constexpr int kPw = 8, kMaxD = 1024 * kPw;
+constexpr int kPw = 8, kPairs = kPw / 2, kMaxD = 1024 * kPw;
 
 struct NrP {
     HdlaNormResidualArgs a;
     int per_row;             // threads of a row (whole warps)
+    int stride;              // floats of a vector in shared memory: kPw * per_row
     float* part;             // backward: [blocks][3][D] (post, pre, scale)
 };
 
-// Two sums over the warps of a row.  `red` has two buffers, used in turn, so that one barrier a sum is enough.
+// Sums over the warps of a row.  `red` has two buffers, used in turn, so that one barrier a sum is enough.
 struct RowSum {
     float2 (*red)[32];
     int turn, first, warps;
-    __device__ __forceinline__ float2 operator()(float a, float b) {
+    __device__ __forceinline__ float one(float a) {
 #pragma unroll
-        for (int o = 16; o; o >>= 1) {
-            a += __shfl_xor_sync(0xffffffffu, a, o);
-            b += __shfl_xor_sync(0xffffffffu, b, o);
-        }
-        if (warps == 1) return make_float2(a, b);
-        if ((threadIdx.x & 31) == 0) red[turn][threadIdx.x >> 5] = make_float2(a, b);
+        for (int o = 16; o; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+        if (warps == 1) return a;
+        float* at = reinterpret_cast<float*>(red[turn]);
+        if ((threadIdx.x & 31) == 0) at[threadIdx.x >> 5] = a;
         __syncthreads();
-        float2 t = make_float2(0.f, 0.f);
-        for (int w = 0; w < warps; ++w) {
-            const float2 v = red[turn][first + w];
-            t.x += v.x; t.y += v.y;
-        }
+        float t = 0.f;
+#pragma unroll 4
+        for (int w = 0; w < warps; ++w) t += at[first + w];
         turn ^= 1;
+        return t;
+    }
+    __device__ __forceinline__ float2 two(float a, float b) {
+        f2 v = f2_pack(a, b);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) v = f2_add(v, __shfl_xor_sync(0xffffffffu, v, o));
+        if (warps > 1) {
+            f2* at = reinterpret_cast<f2*>(red[turn]);
+            if ((threadIdx.x & 31) == 0) at[threadIdx.x >> 5] = v;
+            __syncthreads();
+            v = 0;
+#pragma unroll 4
+            for (int w = 0; w < warps; ++w) v = f2_add(v, at[first + w]);
+            turn ^= 1;
+        }
+        float2 t;
+        f2_unpack(v, t.x, t.y);
         return t;
     }
 };
 
-// Where a thread stands, and its channels' weights.
+// Where a thread stands.
 struct Place {
     int rows, group, col, valid;
     __device__ __forceinline__ explicit Place(const NrP& p) {
@@ -53,23 +71,76 @@ struct Place {
         valid = max(0, min(kPw, p.a.D - col));
     }
 };
-// eight weights: `otherwise` where there is no tensor
-__device__ __forceinline__ void ld_weights(const void* w, int dt, int col, int valid, float otherwise, float (&f)[kPw]) {
+
+// The three vectors of weights in shared memory, `otherwise` where there is no tensor and zero behind the row's end.
+__device__ __forceinline__ void put_weights(const NrP& p, float* to) {
+    for (int i = threadIdx.x; i < p.stride; i += blockDim.x) {
+        const bool in = i < p.a.D;
+        to[i] = !in ? 0.f : p.a.post_weight ? ld_elem(p.a.post_weight, i, p.a.w_dtype) : 1.f;
+        to[p.stride + i] = !in ? 0.f : p.a.pre_weight ? ld_elem(p.a.pre_weight, i, p.a.w_dtype) : 1.f;
+        to[2 * p.stride + i] = !in ? 0.f : p.a.scale ? ld_elem(p.a.scale, i, p.a.w_dtype) : p.a.scale_value;
+    }
+    __syncthreads();
+}
+__device__ __forceinline__ void ld_pairs(const float* at, f2 (&v)[kPairs]) {
 #pragma unroll
-    for (int c = 0; c < kPw; ++c) f[c] = w && c < valid ? ld_elem(w, col + c, dt) : otherwise;
+    for (int i = 0; i < kPairs; i += 2) {
+        const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(at + 2 * i);
+        v[i] = q.x; v[i + 1] = q.y;
+    }
+}
+__device__ __forceinline__ void st_pairs(float* at, const f2 (&v)[kPairs]) {
+#pragma unroll
+    for (int i = 0; i < kPairs; i += 2) *reinterpret_cast<ulonglong2*>(at + 2 * i) = make_ulonglong2(v[i], v[i + 1]);
+}
+template <int DT>
+__device__ __forceinline__ void unpack_pairs(const Pack<DT, kPw>& r, f2 (&v)[kPairs]) {
+    float f[kPw];
+    unpack<DT, kPw>(r, f);
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) v[i] = f2_pack(f[2 * i], f[2 * i + 1]);
+}
+template <int DT, bool Vec>
+__device__ __forceinline__ void st_row(void* base, long long i, int valid, const f2 (&v)[kPairs]) {
+    float f[kPw];
+#pragma unroll
+    for (int c = 0; c < kPairs; ++c) f2_unpack(v[c], f[2 * c], f[2 * c + 1]);
+    st_pack<DT, kPw, Vec>(base, i, valid, f);
 }
 
+// The gate's activation and its derivative.  silu and sigmoid are one expression: s t with t = g or 1, derivative m s + s (1 - s) t
+// with m = 1 or 0.
+struct GateAct {
+    bool plain;
+    f2 m, rest;
+    __device__ __forceinline__ explicit GateAct(int act) : plain(act == HDLA_ACT_NONE) {
+        m = f2_dup(act == HDLA_ACT_SILU ? 1.f : 0.f);
+        rest = f2_dup(act == HDLA_ACT_SILU ? 0.f : 1.f);
+    }
+    __device__ __forceinline__ f2 sigmoid(f2 g) const {
+        float a, b;
+        f2_unpack(g, a, b);
+        return f2_pack(sigmoid_of(a), sigmoid_of(b));
+    }
+    // from g and its sigmoid
+    __device__ __forceinline__ f2 value(f2 g, f2 s) const { return plain ? g : f2_mul(s, f2_fma(g, m, rest)); }
+    __device__ __forceinline__ f2 slope(f2 g, f2 s) const {
+        return plain ? f2_dup(1.f) : f2_fma(f2_fma(s, f2_dup(-1.f), f2_dup(1.f)), f2_mul(s, f2_fma(g, m, rest)), f2_mul(m, s));
+    }
+};
+
 template <int DT, int RDT, bool Vec, int MaxThreads>
-__global__ void __launch_bounds__(MaxThreads) norm_residual_fwd_kernel(const __grid_constant__ NrP p) {
+__global__ void __launch_bounds__(MaxThreads, MaxThreads == 256 ? 4 : MaxThreads == 512 ? 2 : 1)
+norm_residual_fwd_kernel(const __grid_constant__ NrP p) {
+    extern __shared__ __align__(16) float weights[];
     __shared__ float2 red[2][32];
+    put_weights(p, weights);
     const Place at(p);
     const int D = p.a.D;
     RowSum sum{red, 0, at.group * (p.per_row / 32), p.per_row / 32};
-    float post[kPw], pre[kPw], scale[kPw];
-    ld_weights(p.a.post_weight, p.a.w_dtype, at.col, at.valid, 1.f, post);
-    ld_weights(p.a.pre_weight, p.a.w_dtype, at.col, at.valid, 1.f, pre);
-    ld_weights(p.a.scale, p.a.w_dtype, at.col, at.valid, p.a.scale_value, scale);
+    const GateAct act(p.a.activation);
     const float root = sqrtf((float)D);
+    constexpr bool Ahead = MaxThreads <= 512;
     Pack<DT, kPw> nx, ng = {};
     Pack<RDT, kPw> nr = {};
     auto request = [&](long long row) {
@@ -80,51 +151,80 @@ __global__ void __launch_bounds__(MaxThreads) norm_residual_fwd_kernel(const __g
         if (p.a.gate) ng = ld_pack<DT, kPw, Vec>(p.a.gate, i, ok);
     };
     long long first = (long long)blockIdx.x * at.rows;
-    request(first + at.group);
-    for (; first < p.a.rows; first += (long long)gridDim.x * at.rows) {
+    const long long step = (long long)gridDim.x * at.rows;
+    if (Ahead) request(first + at.group);
+    for (; first < p.a.rows; first += step) {
         const long long row = first + at.group;
-        float v[kPw], g[kPw], r[kPw];
-        unpack<DT, kPw>(nx, v);
-        unpack<DT, kPw>(ng, g);
-        unpack<RDT, kPw>(nr, r);
-        request(row + (long long)gridDim.x * at.rows);
+        if (!Ahead) request(row);
+        f2 v[kPairs], g[kPairs], r[kPairs], w[kPairs];
+        unpack_pairs<DT>(nx, v);
+        unpack_pairs<DT>(ng, g);
+        unpack_pairs<RDT>(nr, r);
+        if (Ahead) request(row + step);
         if (p.a.post_weight) {
-            float ss = 0.f;
+            f2 ss = 0;
 #pragma unroll
-            for (int c = 0; c < kPw; ++c) ss = fmaf(v[c], v[c], ss);
-            const float k = root * rsqrtf(sum(ss, 0.f).x + p.a.eps);
+            for (int c = 0; c < kPairs; ++c) ss = f2_fma(v[c], v[c], ss);
+            const f2 k = f2_dup(root * rsqrtf(sum.one(f2_sum(ss)) + p.a.eps));
+            ld_pairs(weights + at.col, w);
 #pragma unroll
-            for (int c = 0; c < kPw; ++c) v[c] *= k * post[c];
+            for (int c = 0; c < kPairs; ++c) v[c] = f2_mul(v[c], f2_mul(k, w[c]));
         }
-        float ss = 0.f;
+        if (p.a.gate)
 #pragma unroll
-        for (int c = 0; c < kPw; ++c) {
-            if (p.a.gate) v[c] *= act_of(g[c], p.a.activation);
-            r[c] = fmaf(scale[c], v[c], r[c]);
-            if (c < at.valid) ss = fmaf(r[c], r[c], ss);
+            for (int c = 0; c < kPairs; ++c) v[c] = f2_mul(v[c], act.value(g[c], act.sigmoid(g[c])));
+        ld_pairs(weights + 2 * p.stride + at.col, w);
+        f2 ss = 0;
+#pragma unroll
+        for (int c = 0; c < kPairs; ++c) {
+            r[c] = f2_fma(w[c], v[c], r[c]);
+            ss = f2_fma(r[c], r[c], ss);
         }
         const int ok = row < p.a.rows ? at.valid : 0;
-        st_pack<RDT, kPw, Vec>(p.a.r, row * D + at.col, ok, r);
+        st_row<RDT, Vec>(p.a.r, row * D + at.col, ok, r);
         if (p.a.pre_weight) {
-            const float k = root * rsqrtf(sum(ss, 0.f).x + p.a.eps);
+            const f2 k = f2_dup(root * rsqrtf(sum.one(f2_sum(ss)) + p.a.eps));
+            ld_pairs(weights + p.stride + at.col, w);
 #pragma unroll
-            for (int c = 0; c < kPw; ++c) r[c] *= k * pre[c];
-            st_pack<DT, kPw, Vec>(p.a.u, row * D + at.col, ok, r);
+            for (int c = 0; c < kPairs; ++c) r[c] = f2_mul(r[c], f2_mul(k, w[c]));
+            st_row<DT, Vec>(p.a.u, row * D + at.col, ok, r);
         }
     }
 }
 
 template <int DT, int RDT, bool Vec, int MaxThreads>
-__global__ void __launch_bounds__(MaxThreads) norm_residual_bwd_kernel(const __grid_constant__ NrP p) {
+__global__ void __launch_bounds__(MaxThreads, MaxThreads == 256 ? 2 : 1) norm_residual_bwd_kernel(const __grid_constant__ NrP p) {
+    extern __shared__ __align__(16) float weights[];        // 3 vectors; 3 of sums behind them where those are not in registers
     __shared__ float2 red[2][32];
-    __shared__ float over[kPw * 256];                       // rows that share a block (at most 256 threads then)
+    constexpr bool Lean = MaxThreads > 512;
+    put_weights(p, weights);
     const Place at(p);
     const int D = p.a.D;
     RowSum sum{red, 0, at.group * (p.per_row / 32), p.per_row / 32};
-    float post[kPw], pre[kPw], scale[kPw], dpost[kPw] = {}, dpre[kPw] = {}, dscale[kPw] = {};
-    ld_weights(p.a.post_weight, p.a.w_dtype, at.col, at.valid, 1.f, post);
-    ld_weights(p.a.pre_weight, p.a.w_dtype, at.col, at.valid, 1.f, pre);
-    ld_weights(p.a.scale, p.a.w_dtype, at.col, at.valid, p.a.scale_value, scale);
+    const GateAct act(p.a.activation);
+    f2 acc[Lean ? 1 : 3][kPairs];                           // post, pre, scale
+    float* sums = weights + 3 * p.stride + at.col;
+#pragma unroll
+    for (int c = 0; c < kPairs; ++c) acc[0][c] = 0;
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+        if (Lean) st_pairs(sums + k * p.stride, acc[0]);
+        else
+#pragma unroll
+            for (int c = 0; c < kPairs; ++c) acc[Lean ? 0 : k][c] = 0;
+    }
+    auto add = [&](int k, const f2 (&a)[kPairs], const f2 (&b)[kPairs]) {      // sum k += a b
+        if constexpr (Lean) {
+            f2 t[kPairs];
+            ld_pairs(sums + k * p.stride, t);
+#pragma unroll
+            for (int c = 0; c < kPairs; ++c) t[c] = f2_fma(a[c], b[c], t[c]);
+            st_pairs(sums + k * p.stride, t);
+        } else {
+#pragma unroll
+            for (int c = 0; c < kPairs; ++c) acc[k][c] = f2_fma(a[c], b[c], acc[k][c]);
+        }
+    };
     const float root = sqrtf((float)D), per = 1.f / (float)D;
     Pack<DT, kPw> nx, ng = {}, nu = {};
     Pack<RDT, kPw> nr = {}, nd = {};
@@ -138,91 +238,120 @@ __global__ void __launch_bounds__(MaxThreads) norm_residual_bwd_kernel(const __g
         if (p.a.du) nu = ld_pack<DT, kPw, Vec>(p.a.du, i, ok);
     };
     long long first = (long long)blockIdx.x * at.rows;
-    request(first + at.group);
-    for (; first < p.a.rows; first += (long long)gridDim.x * at.rows) {
+    const long long step = (long long)gridDim.x * at.rows;
+    if (!Lean) request(first + at.group);
+    for (; first < p.a.rows; first += step) {
         const long long row = first + at.group;
-        float x[kPw], g[kPw], d[kPw];
-        unpack<DT, kPw>(nx, x);
-        unpack<DT, kPw>(ng, g);
-        unpack<RDT, kPw>(nd, d);
-        const Pack<RDT, kPw> cr = nr;
-        const Pack<DT, kPw> cu = nu;
-        request(row + (long long)gridDim.x * at.rows);
+        if (Lean) request(row);
+        const Pack<DT, kPw> cx = nx, cg = ng, cu = nu;
+        const Pack<RDT, kPw> cr = nr, cd = nd;
+        if (!Lean) request(row + step);
+        const bool exists = row < p.a.rows;                 // (a block's last rows may not)
+        // what is used twice is unpacked twice: registers are short
+        f2 s[kPairs], d[kPairs];                            // the gate's sigmoid; the gradient on its way from r to x
         float kx = 1.f;                                     // n = x kx post, v = n act(g), r = residual + scale v
         if (p.a.post_weight) {
-            float ss = 0.f;
+            f2 x[kPairs], ss = 0;
+            unpack_pairs<DT>(cx, x);
 #pragma unroll
-            for (int c = 0; c < kPw; ++c) ss = fmaf(x[c], x[c], ss);
-            ss = sum(ss, 0.f).x;
-            kx = row < p.a.rows ? root * rsqrtf(ss + p.a.eps) : 0.f;      // (a block's last rows may not exist)
+            for (int c = 0; c < kPairs; ++c) ss = f2_fma(x[c], x[c], ss);
+            const float t = sum.one(f2_sum(ss));
+            kx = exists ? root * rsqrtf(t + p.a.eps) : 0.f;
         }
+        if (p.a.gate) {
+            unpack_pairs<DT>(cg, s);
+#pragma unroll
+            for (int c = 0; c < kPairs; ++c) s[c] = act.sigmoid(s[c]);
+        }
+        unpack_pairs<RDT>(cd, d);
         if (p.a.pre_weight) {
-            float r[kPw], t[kPw], ss = 0.f, dot = 0.f;
-            unpack<RDT, kPw>(cr, r);
-            unpack<DT, kPw>(cu, t);
+            f2 x[kPairs], r[kPairs], w[kPairs], k[kPairs], ss = 0, dot = 0;
+            unpack_pairs<DT>(cx, x);
+            ld_pairs(weights + at.col, w);
 #pragma unroll
-            for (int c = 0; c < kPw; ++c) {
-                float v = x[c] * kx * post[c];
-                if (p.a.gate) v *= act_of(g[c], p.a.activation);
-                r[c] = fmaf(scale[c], v, r[c]);
-                if (c < at.valid) {
-                    ss = fmaf(r[c], r[c], ss);
-                    dot = fmaf(t[c] * pre[c], r[c], dot);
-                }
-            }
-            const float2 s = sum(ss, dot);
-            const float kr = row < p.a.rows ? root * rsqrtf(s.x + p.a.eps) : 0.f, back = kr * kr * kr * per * s.y;
-#pragma unroll
-            for (int c = 0; c < kPw; ++c) {
-                d[c] += kr * (t[c] * pre[c]) - back * r[c];
-                dpre[c] = fmaf(t[c] * kr, r[c], dpre[c]);
-            }
-        }
-        const int ok = row < p.a.rows ? at.valid : 0;
-        const long long i = row * D + at.col;
-        if (p.a.dresidual) st_pack<RDT, kPw, Vec>(p.a.dresidual, i, ok, d);
-        float dot = 0.f;
-#pragma unroll
-        for (int c = 0; c < kPw; ++c) {
-            const float n = x[c] * kx * post[c];
-            float v = n, dv = scale[c] * d[c];
+            for (int c = 0; c < kPairs; ++c) x[c] = f2_mul(x[c], f2_mul(w[c], f2_dup(kx)));
             if (p.a.gate) {
-                const float act = act_of(g[c], p.a.activation);
-                v *= act;
-                g[c] = dv * n * act_grad(g[c], p.a.activation);
-                dv *= act;
-            }
-            dscale[c] = fmaf(d[c], v, dscale[c]);
-            d[c] = dv;
-            dot = fmaf(dv * post[c], x[c], dot);
-        }
-        if (p.a.dgate) st_pack<DT, kPw, Vec>(p.a.dgate, i, ok, g);
-        if (p.a.post_weight) {
-            const float back = kx * kx * kx * per * sum(dot, 0.f).x;
+                f2 g[kPairs];
+                unpack_pairs<DT>(cg, g);
 #pragma unroll
-            for (int c = 0; c < kPw; ++c) {
-                dpost[c] = fmaf(d[c] * kx, x[c], dpost[c]);
-                d[c] = kx * (d[c] * post[c]) - back * x[c];
+                for (int c = 0; c < kPairs; ++c) x[c] = f2_mul(x[c], act.value(g[c], s[c]));
             }
+            unpack_pairs<RDT>(cr, r);
+            ld_pairs(weights + 2 * p.stride + at.col, k);
+            ld_pairs(weights + p.stride + at.col, w);
+            f2 t[kPairs];
+            unpack_pairs<DT>(cu, t);
+#pragma unroll
+            for (int c = 0; c < kPairs; ++c) {
+                r[c] = f2_fma(k[c], x[c], r[c]);
+                ss = f2_fma(r[c], r[c], ss);
+                dot = f2_fma(f2_mul(t[c], w[c]), r[c], dot);
+            }
+            const float2 both = sum.two(f2_sum(ss), f2_sum(dot));
+            const float kr = exists ? root * rsqrtf(both.x + p.a.eps) : 0.f, back = kr * kr * kr * per * both.y;
+#pragma unroll
+            for (int c = 0; c < kPairs; ++c) {
+                t[c] = f2_mul(t[c], f2_dup(kr));
+                d[c] = f2_fma(t[c], w[c], f2_fma(f2_dup(-back), r[c], d[c]));
+            }
+            add(1, t, r);
         }
-        st_pack<DT, kPw, Vec>(p.a.dx, i, ok, d);
+        const int ok = exists ? at.valid : 0;
+        const long long i = row * D + at.col;
+        if (p.a.dresidual) st_row<RDT, Vec>(p.a.dresidual, i, ok, d);
+        f2 x[kPairs], w[kPairs];
+        unpack_pairs<DT>(cx, x);
+        ld_pairs(weights + at.col, w);
+        {
+            f2 n[kPairs], k[kPairs];
+#pragma unroll
+            for (int c = 0; c < kPairs; ++c) n[c] = f2_mul(x[c], f2_mul(w[c], f2_dup(kx)));
+            ld_pairs(weights + 2 * p.stride + at.col, k);
+            if (p.a.gate) {
+                f2 g[kPairs], v[kPairs];
+                unpack_pairs<DT>(cg, g);
+#pragma unroll
+                for (int c = 0; c < kPairs; ++c) {
+                    const f2 a = act.value(g[c], s[c]), dv = f2_mul(k[c], d[c]);
+                    v[c] = f2_mul(n[c], a);
+                    g[c] = f2_mul(f2_mul(dv, n[c]), act.slope(g[c], s[c]));
+                    k[c] = f2_mul(dv, a);
+                }
+                add(2, d, v);
+                if (p.a.dgate) st_row<DT, Vec>(p.a.dgate, i, ok, g);
+            } else {
+                add(2, d, n);
+#pragma unroll
+                for (int c = 0; c < kPairs; ++c) k[c] = f2_mul(k[c], d[c]);
+            }
+#pragma unroll
+            for (int c = 0; c < kPairs; ++c) d[c] = k[c];
+        }
+        if (p.a.post_weight) {
+            f2 dot = 0;
+#pragma unroll
+            for (int c = 0; c < kPairs; ++c) dot = f2_fma(f2_mul(d[c], w[c]), x[c], dot);
+            const float back = kx * kx * kx * per * sum.one(f2_sum(dot));
+#pragma unroll
+            for (int c = 0; c < kPairs; ++c) d[c] = f2_mul(d[c], f2_dup(kx));
+            add(0, d, x);
+#pragma unroll
+            for (int c = 0; c < kPairs; ++c) d[c] = f2_fma(d[c], w[c], f2_mul(f2_dup(-back), x[c]));
+        }
+        st_row<DT, Vec>(p.a.dx, i, ok, d);
     }
 #pragma unroll
-    for (int what = 0; what < 3; ++what) {
-        const float* s = what == 0 ? dpost : what == 1 ? dpre : dscale;
-        float* to = p.part + ((long long)blockIdx.x * 3 + what) * D;
-        if (at.rows == 1) {
-#pragma unroll
-            for (int c = 0; c < kPw; ++c)
-                if (c < at.valid) to[at.col + c] = s[c];
+    for (int k = 0; k < 3; ++k) {
+        float* to = p.part + ((long long)blockIdx.x * 3 + k) * D;
+        __syncthreads();                                    // (the weights are not read any more, nor the sums before)
+        if (Lean) {
+            for (int c = threadIdx.x; c < D; c += blockDim.x) to[c] = weights[(3 + k) * p.stride + c];
         } else {
-            __syncthreads();
-#pragma unroll
-            for (int c = 0; c < kPw; ++c) over[threadIdx.x * kPw + c] = s[c];
+            st_pairs(weights + at.group * p.stride + at.col, acc[Lean ? 0 : k]);
             __syncthreads();
             for (int c = threadIdx.x; c < D; c += blockDim.x) {
                 float v = 0.f;
-                for (int k = 0; k < at.rows; ++k) v += over[k * p.per_row * kPw + c];
+                for (int g = 0; g < at.rows; ++g) v += weights[g * p.stride + c];
                 to[c] = v;
             }
         }
@@ -252,11 +381,30 @@ Kernel pick(const HdlaNormResidualArgs& a, bool backward, int threads) {
     if (a.r_dtype == HDLA_F32) return vec ? kernel_for<HDLA_BF16, HDLA_F32, true>(backward, threads) : kernel_for<HDLA_BF16, HDLA_F32, false>(backward, threads);
     return vec ? kernel_for<HDLA_BF16, HDLA_BF16, true>(backward, threads) : kernel_for<HDLA_BF16, HDLA_BF16, false>(backward, threads);
 }
-// as many blocks as there are rows for, and at most four (backward: two) of 256 threads an SM, which walk over the rows
+// as many blocks as there are rows for, and at most those that are resident at once (four of 256 threads an SM, two backward);
+// they walk over the rows
 unsigned blocks_of(const HdlaNormResidualArgs& a, bool backward) {
     const int per_row = row_threads(a.D), threads = block_threads(per_row), rows = threads / per_row;
-    const long long need = (a.rows + rows - 1) / rows, most = (long long)sm_count() * ((backward ? 512 : 1024) / threads > 1 ? (backward ? 512 : 1024) / threads : 1);
+    const long long need = (a.rows + rows - 1) / rows, each = (backward ? 512 : 1024) / threads, most = (long long)sm_count() * (each > 1 ? each : 1);
     return static_cast<unsigned>(need < most ? need : most);
+}
+// three vectors of weights, which at the end make room for a vector of sums for each row of the block; three more of sums
+size_t shared_of(int per_row, int threads, bool backward) {
+    const int rows = threads / per_row, vectors = !backward ? 3 : threads > 512 ? 6 : rows > 3 ? rows : 3;
+    return sizeof(float) * kPw * per_row * vectors;
+}
+int launch(const HdlaNormResidualArgs& a, bool backward, float* part, cudaStream_t st) {
+    const int per_row = row_threads(a.D), threads = block_threads(per_row);
+    const NrP p{a, per_row, kPw * per_row, part};
+    const Kernel kernel = pick(a, backward, threads);
+    const size_t bytes = shared_of(per_row, threads, backward);
+    if (bytes > 47 << 10) {                                      // (the sums have some of the 48 KB that need no request)
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+        if (e != cudaSuccess) return fail(HDLA_ERR_CUDA, "norm_residual: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+    }
+    kernel<<<blocks_of(a, backward), threads, bytes, st>>>(p);
+    HDLA_CHECK_LAUNCH(backward ? "norm_residual_bwd_kernel" : "norm_residual_fwd_kernel");
+    return HDLA_OK;
 }
 
 }  // namespace
@@ -265,24 +413,14 @@ int norm_residual_max_d() { return kMaxD; }
 
 size_t norm_residual_bwd_workspace(const HdlaNormResidualArgs& a) { return up256((size_t)blocks_of(a, true) * 3 * a.D * sizeof(float)); }
 
-int norm_residual_fwd(const HdlaNormResidualArgs& a, cudaStream_t st) {
-    NrP p{a, row_threads(a.D), nullptr};
-    const int threads = block_threads(p.per_row);
-    pick(a, false, threads)<<<blocks_of(a, false), threads, 0, st>>>(p);
-    HDLA_CHECK_LAUNCH("norm_residual_fwd_kernel");
-    return HDLA_OK;
-}
+int norm_residual_fwd(const HdlaNormResidualArgs& a, cudaStream_t st) { return launch(a, false, nullptr, st); }
 
 int norm_residual_bwd(const HdlaNormResidualArgs& a, float* part, cudaStream_t st) {
-    NrP p{a, row_threads(a.D), part};
-    const int threads = block_threads(p.per_row);
-    const unsigned blocks = blocks_of(a, true);
-    pick(a, true, threads)<<<blocks, threads, 0, st>>>(p);
-    HDLA_CHECK_LAUNCH("norm_residual_bwd_kernel");
+    if (int rc = launch(a, true, part, st)) return rc;
     if (!a.dpost_weight && !a.dpre_weight && !a.dscale) return HDLA_OK;
     ColJobs js{};
     js.n = 1;
-    js.j[0] = ColJob{part, {a.dpost_weight, a.dpre_weight, a.dscale}, 3LL * a.D, (int)blocks, 3, a.D, a.D, a.w_dtype, 0, 0, 0};
+    js.j[0] = ColJob{part, {a.dpost_weight, a.dpre_weight, a.dscale}, 3LL * a.D, (int)blocks_of(a, true), 3, a.D, a.D, a.w_dtype, 0, 0, 0};
     return column_sum_launch(js, st);
 }
 

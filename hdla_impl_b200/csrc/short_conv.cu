@@ -1,13 +1,20 @@
 // Depthwise causal convolution over W taps with its activation:
 //     p_t = bias + sum_{k<W} w[W-1-k] x_{t-k},   y_t = act(p_t)
 // forward, backward and the step of single tokens.  A handful of operations an element: bound by HBM (x in, y out; backward x
-// and dy in, dx out).  A thread owns PW neighbouring channels (one 16-byte access of x forward, 8 bytes of bf16 backward, where
-// the taps' sums need the registers) and walks over a strip of tokens with the last W - 1 inputs in registers, so that a row
-// is read once, plus W - 1 rows at each strip's edge, which the neighbouring strip has just brought to L2.
+// and dy in, dx out).  A thread owns four neighbouring channels, as two packed pairs, and walks over a strip of tokens with the
+// last W - 1 inputs in registers, so that a row is read once, plus W - 1 rows at each strip's edge, which the neighbouring strip
+// has just brought to L2.  Several tokens are requested at a time, and forward the next ones before these are worked on.  Four
+// channels a thread and not eight (16 bytes of bf16): the taps, their sums and the histories are what fills the registers, and
+// with half of them twice the warps hide the latency (forward 100 -> 57 us, backward 262 -> 128 us at 32768 x 2048, W = 4).
+#include "f32x2.cuh"
 #include "ssm.cuh"
 
 namespace hdla {
 namespace {
+
+constexpr int PW = 4;
+constexpr int kFwdWarps = 4, kBwdWarps = 8;
+struct Quad { f2 v[2]; };                                        // four channels
 
 struct ConvP {
     HdlaConvArgs a;
@@ -18,73 +25,85 @@ struct ConvP {
 };
 
 template <int DT>
-__device__ __forceinline__ constexpr int pack_width() { return DT == HDLA_F32 ? 4 : 8; }
+__device__ __forceinline__ Quad quad_of(const Pack<DT, PW>& r) {
+    float f[PW];
+    unpack<DT, PW>(r, f);
+    return Quad{{f2_pack(f[0], f[1]), f2_pack(f[2], f[3])}};
+}
+template <int DT, bool Vec>
+__device__ __forceinline__ void st_quad(void* base, long long i, int valid, const Quad& q) {
+    float f[PW];
+    f2_unpack(q.v[0], f[0], f[1]);
+    f2_unpack(q.v[1], f[2], f[3]);
+    st_pack<DT, PW, Vec>(base, i, valid, f);
+}
+__device__ __forceinline__ f2 sigmoid_pair(f2 v) {
+    float a, b;
+    f2_unpack(v, a, b);
+    return f2_pack(sigmoid_of(a), sigmoid_of(b));
+}
 
-// w[k][c]: the weight of lag k for channel c of the thread's PW
-template <int PW, int WT, bool Vec>
-__device__ __forceinline__ void load_taps(const ConvP& p, int ch, int valid, float (&w)[WT][PW], float (&bias)[PW]) {
+// w[k]: the weights of lag k for the thread's channels
+template <int WT, bool Vec>
+__device__ __forceinline__ void load_taps(const ConvP& p, int ch, int valid, Quad (&w)[WT], Quad& bias) {
     const int W = WT == 8 ? p.a.W : WT;
+    float f[PW][WT], b[PW];
     bool done = false;
-    if constexpr (Vec && WT != 8) {
-        if (p.wide_w && valid > 0) {
-            if (p.a.w_dtype == HDLA_BF16) {
-                if constexpr (PW * WT % 8 == 0) {
-                    Pack<HDLA_BF16, PW * WT> r = ld_pack<HDLA_BF16, PW * WT, true>(p.a.weight, (long long)ch * WT, 1);
-                    float f[PW * WT];
-                    unpack<HDLA_BF16, PW * WT>(r, f);
-#pragma unroll
-                    for (int c = 0; c < PW; ++c)
-#pragma unroll
-                        for (int k = 0; k < WT; ++k) w[k][c] = f[c * WT + WT - 1 - k];
-                    done = true;
-                }
-            } else if constexpr (PW * WT % 4 == 0) {
-                Pack<HDLA_F32, PW * WT> r = ld_pack<HDLA_F32, PW * WT, true>(p.a.weight, (long long)ch * WT, 1);
-#pragma unroll
-                for (int c = 0; c < PW; ++c)
-#pragma unroll
-                    for (int k = 0; k < WT; ++k) w[k][c] = __uint_as_float(r.w[c * WT + WT - 1 - k]);
-                done = true;
-            }
+    if constexpr (Vec && WT != 8 && PW * WT % 8 == 0) {
+        if (p.wide_w) {
+            if (p.a.w_dtype == HDLA_BF16)
+                unpack<HDLA_BF16, PW * WT>(ld_pack<HDLA_BF16, PW * WT, true>(p.a.weight, (long long)ch * WT, 1), &f[0][0]);
+            else
+                unpack<HDLA_F32, PW * WT>(ld_pack<HDLA_F32, PW * WT, true>(p.a.weight, (long long)ch * WT, 1), &f[0][0]);
+            done = true;
         }
     }
 #pragma unroll
     for (int c = 0; c < PW; ++c) {
         if (!done)
 #pragma unroll
-            for (int k = 0; k < WT; ++k)
-                w[k][c] = c < valid && k < W ? ld_elem(p.a.weight, (size_t)(ch + c) * W + (W - 1 - k), p.a.w_dtype) : 0.f;
-        bias[c] = p.a.bias && c < valid ? ld_elem(p.a.bias, ch + c, p.a.w_dtype) : 0.f;
+            for (int j = 0; j < WT; ++j) f[c][j] = c < valid && j < W ? ld_elem(p.a.weight, (size_t)(ch + c) * W + j, p.a.w_dtype) : 0.f;
+        b[c] = p.a.bias && c < valid ? ld_elem(p.a.bias, ch + c, p.a.w_dtype) : 0.f;
     }
+#pragma unroll
+    for (int k = 0; k < WT; ++k) {
+        float t[PW];
+#pragma unroll
+        for (int c = 0; c < PW; ++c) {
+            t[c] = 0.f;
+#pragma unroll
+            for (int j = 0; j < WT; ++j)
+                if (WT != 8 ? j == WT - 1 - k : j == W - 1 - k) t[c] = f[c][j];
+        }
+        w[k] = Quad{{f2_pack(t[0], t[1]), f2_pack(t[2], t[3])}};
+    }
+    bias = Quad{{f2_pack(b[0], b[1]), f2_pack(b[2], b[3])}};
 }
 
 // Taps beyond W (only with WT == 8) are left out, not multiplied by zero: what they would read may be infinite.
-template <int PW, int WT>
-__device__ __forceinline__ void taps(const float (&w)[WT][PW], const float (&bias)[PW], const float* x, const float (&hist)[WT - 1][PW],
-                                     int W, float* out) {
+template <int WT>
+__device__ __forceinline__ Quad taps(const Quad (&w)[WT], const Quad& bias, const Quad& x, const Quad (&hist)[WT - 1], int W) {
+    Quad out;
 #pragma unroll
-    for (int c = 0; c < PW; ++c) {
-        float s = fmaf(w[0][c], x[c], bias[c]);
+    for (int c = 0; c < 2; ++c) {
+        f2 s = f2_fma(w[0].v[c], x.v[c], bias.v[c]);
 #pragma unroll
         for (int k = 1; k < WT; ++k)
-            if (WT != 8 || k < W) s = fmaf(w[k][c], hist[k - 1][c], s);
-        out[c] = s;
+            if (WT != 8 || k < W) s = f2_fma(w[k].v[c], hist[k - 1].v[c], s);
+        out.v[c] = s;
     }
+    return out;
 }
-template <int PW, int N>
-__device__ __forceinline__ void shift(float (&hist)[N][PW], const float* x) {
+template <int N>
+__device__ __forceinline__ void shift(Quad (&hist)[N], const Quad& x) {
 #pragma unroll
-    for (int k = N - 1; k > 0; --k)
-#pragma unroll
-        for (int c = 0; c < PW; ++c) hist[k][c] = hist[k - 1][c];
-#pragma unroll
-    for (int c = 0; c < PW; ++c) hist[0][c] = x[c];
+    for (int k = N - 1; k > 0; --k) hist[k] = hist[k - 1];
+    hist[0] = x;
 }
 
 // The inputs of the W - 1 tokens before token t of a sequence that starts at `start`: its initial state's rows before that.
-template <int DT, int PW, int WT, bool Vec>
-__device__ __forceinline__ void load_hist(const ConvP& p, long long xrow, long long state, int start, int t, int ch, int valid,
-                                          float (&hist)[WT - 1][PW]) {
+template <int DT, int WT, bool Vec>
+__device__ __forceinline__ void load_hist(const ConvP& p, long long xrow, long long state, int start, int t, int ch, int valid, Quad (&hist)[WT - 1]) {
     const int W = WT == 8 ? p.a.W : WT;
 #pragma unroll
     for (int k = 0; k < WT - 1; ++k) {
@@ -94,22 +113,20 @@ __device__ __forceinline__ void load_hist(const ConvP& p, long long xrow, long l
             if (tt >= start) r = ld_pack<DT, PW, Vec>(p.a.x, xrow + tt * p.a.x_token + ch, valid);
             else if (p.a.h0) r = ld_pack<DT, PW, Vec>(p.a.h0, (state * (W - 1) + (W - 1 + tt - start)) * p.a.D + ch, valid);
         }
-        unpack<DT, PW>(r, hist[k]);
+        hist[k] = quad_of<DT>(r);
     }
 }
-template <int DT, int PW, int WT, bool Vec>
-__device__ __forceinline__ void store_state(const ConvP& p, void* to, long long state, int ch, int valid, const float (&hist)[WT - 1][PW]) {
+template <int DT, int WT, bool Vec>
+__device__ __forceinline__ void store_state(const ConvP& p, long long state, int ch, int valid, const Quad (&hist)[WT - 1]) {
     const int W = WT == 8 ? p.a.W : WT;
 #pragma unroll
     for (int k = 0; k < WT - 1; ++k)
-        if (k < W - 1) st_pack<DT, PW, Vec>(to, (state * (W - 1) + (W - 2 - k)) * p.a.D + ch, valid, hist[k]);
+        if (k < W - 1) st_quad<DT, Vec>(p.a.ht, (state * (W - 1) + (W - 2 - k)) * p.a.D + ch, valid, hist[k]);
 }
-
-constexpr int kFwdWarps = 4, kBwdWarps = 8;
 
 template <int DT, int WT, bool Vec>
 __global__ void __launch_bounds__(32 * kFwdWarps) conv_fwd_kernel(const __grid_constant__ ConvP p) {
-    constexpr int PW = pack_width<DT>(), U = 8;
+    constexpr int U = 4;
     const int T = p.a.T, D = p.a.D, W = WT == 8 ? p.a.W : WT;
     const int cb = blockIdx.x % p.col_blocks, sb = blockIdx.x / p.col_blocks % p.strips, b = blockIdx.x / p.col_blocks / p.strips;
     const int ch = (cb * 32 + (threadIdx.x & 31)) * PW, valid = min(PW, D - ch);
@@ -117,69 +134,86 @@ __global__ void __launch_bounds__(32 * kFwdWarps) conv_fwd_kernel(const __grid_c
     if (valid <= 0 || first >= T) return;
     const int t0 = static_cast<int>(first), t1 = min(T, t0 + p.strip);
     const Seqs q{p.a.cu_seqlens, p.a.cu_seqlens ? p.a.n_seqs : 1, T};
-    const long long xrow = b * p.a.x_batch, yrow = (long long)b * T;
-    float w[WT][PW], bias[PW], hist[WT - 1][PW];
-    load_taps<PW, WT, Vec>(p, ch, valid, w, bias);
+    const long long xrow = b * p.a.x_batch;
+    constexpr int size = DT == HDLA_F32 ? 4 : 2;
+    const char* from = static_cast<const char*>(p.a.x) + (xrow + t0 * p.a.x_token + ch) * size;
+    char* to = static_cast<char*>(p.a.y) + (((long long)b * T + t0) * D + ch) * size;
+    const long long from_step = p.a.x_token * size, to_step = (long long)D * size;
+    Pack<DT, PW> in[U], next[U];
+    auto request = [&](int tokens) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) next[u] = ld_pack<DT, PW, Vec>(from + u * from_step, 0, u < tokens ? valid : 0);
+        from += U * from_step;
+    };
+    request(t1 - t0);
+    Quad w[WT], bias, hist[WT - 1];
+    load_taps<WT, Vec>(p, ch, valid, w, bias);
     int s = q.ends_behind(t0);
     if (t0 == 0 && p.a.ht)
         for (int i = 0; i < s; ++i) {                          // empty sequences at the front
-            load_hist<DT, PW, WT, Vec>(p, xrow, b + i, 0, 0, ch, valid, hist);
-            store_state<DT, PW, WT, Vec>(p, p.a.ht, b + i, ch, valid, hist);
+            load_hist<DT, WT, Vec>(p, xrow, b + i, 0, 0, ch, valid, hist);
+            store_state<DT, WT, Vec>(p, b + i, ch, valid, hist);
         }
     int end = s < q.n ? q.off(s + 1) : 0x7fffffff;
-    if (s < q.n) load_hist<DT, PW, WT, Vec>(p, xrow, b + s, min(q.off(s), t0), t0, ch, valid, hist);
+    load_hist<DT, WT, Vec>(p, xrow, b + min(s, q.n - 1), s < q.n ? min(q.off(s), t0) : t0, t0, ch, valid, hist);
     for (int t = t0; t < t1; t += U) {
-        Pack<DT, PW> in[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (t + u < t1) in[u] = ld_pack<DT, PW, Vec>(p.a.x, xrow + (t + u) * p.a.x_token + ch, valid);
+        for (int u = 0; u < U; ++u) in[u] = next[u];
+        if (t + U < t1) request(t1 - t - U);
+        auto one = [&](int u) {
+            const Quad x = quad_of<DT>(in[u]);
+            Quad out = taps<WT>(w, bias, x, hist, W);
+            if (p.a.activation == HDLA_ACT_SILU)
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (t + u >= t1) break;
-            float x[PW], out[PW];
-            unpack<DT, PW>(in[u], x);
-            taps<PW, WT>(w, bias, x, hist, W, out);
+                for (int c = 0; c < 2; ++c) out.v[c] = f2_mul(out.v[c], sigmoid_pair(out.v[c]));
+            shift(hist, x);
+            return out;
+        };
+        if (t + U <= t1 && end > t + U && s < q.n) {
 #pragma unroll
-            for (int c = 0; c < PW; ++c) {
-                if (p.a.activation == HDLA_ACT_SILU) out[c] *= sigmoid_of(out[c]);
-                if (s >= q.n) out[c] = 0.f;
-            }
-            st_pack<DT, PW, Vec>(p.a.y, (yrow + t + u) * D + ch, valid, out);
-            shift<PW, WT - 1>(hist, x);
-            while (end <= t + u + 1) {                         // this token was a sequence's last (and empty ones follow)
-                if (p.a.ht) store_state<DT, PW, WT, Vec>(p, p.a.ht, b + s, ch, valid, hist);
-                if (++s < q.n) {
-                    load_hist<DT, PW, WT, Vec>(p, xrow, b + s, t + u + 1, t + u + 1, ch, valid, hist);
-                    end = q.off(s + 1);
-                } else {
-                    end = 0x7fffffff;
+            for (int u = 0; u < U; ++u) st_quad<DT, Vec>(to + u * to_step, 0, valid, one(u));
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (t + u >= t1) break;
+                Quad out = one(u);
+                if (s >= q.n) out = Quad{{0, 0}};              // a token of no sequence
+                st_quad<DT, Vec>(to + u * to_step, 0, valid, out);
+                while (end <= t + u + 1) {                     // this token was a sequence's last (and empty ones follow)
+                    if (p.a.ht) store_state<DT, WT, Vec>(p, b + s, ch, valid, hist);
+                    if (++s < q.n) {
+                        load_hist<DT, WT, Vec>(p, xrow, b + s, t + u + 1, t + u + 1, ch, valid, hist);
+                        end = q.off(s + 1);
+                    } else {
+                        end = 0x7fffffff;
+                    }
                 }
             }
         }
+        to += U * to_step;
     }
 }
 
 // One token: the state is the history, and moves on by one row in place (a thread owns its channels' rows).
 template <int DT, int WT, bool Vec>
 __global__ void __launch_bounds__(128) conv_step_kernel(const __grid_constant__ ConvP p) {
-    constexpr int PW = pack_width<DT>();
     const int D = p.a.D, W = WT == 8 ? p.a.W : WT;
     const int cb = blockIdx.x % p.col_blocks;
     const long long b = (long long)(blockIdx.x / p.col_blocks) * 4 + (threadIdx.x >> 5);
     const int ch = (cb * 32 + (threadIdx.x & 31)) * PW, valid = min(PW, D - ch);
     if (valid <= 0 || b >= p.a.B) return;
-    float w[WT][PW], bias[PW], hist[WT - 1][PW], x[PW], out[PW];
+    Quad w[WT], bias, hist[WT - 1];
     const Pack<DT, PW> in = ld_pack<DT, PW, Vec>(p.a.x, b * p.a.x_batch + ch, valid);
-    load_hist<DT, PW, WT, Vec>(p, 0, b, 0, 0, ch, valid, hist);
-    load_taps<PW, WT, Vec>(p, ch, valid, w, bias);
-    unpack<DT, PW>(in, x);
-    taps<PW, WT>(w, bias, x, hist, W, out);
+    load_hist<DT, WT, Vec>(p, 0, b, 0, 0, ch, valid, hist);
+    load_taps<WT, Vec>(p, ch, valid, w, bias);
+    const Quad x = quad_of<DT>(in);
+    Quad out = taps<WT>(w, bias, x, hist, W);
     if (p.a.activation == HDLA_ACT_SILU)
 #pragma unroll
-        for (int c = 0; c < PW; ++c) out[c] *= sigmoid_of(out[c]);
-    st_pack<DT, PW, Vec>(p.a.y, b * D + ch, valid, out);
-    shift<PW, WT - 1>(hist, x);
-    store_state<DT, PW, WT, Vec>(p, p.a.ht, b, ch, valid, hist);
+        for (int c = 0; c < 2; ++c) out.v[c] = f2_mul(out.v[c], sigmoid_pair(out.v[c]));
+    st_quad<DT, Vec>(p.a.y, b * D + ch, valid, out);
+    shift(hist, x);
+    store_state<DT, WT, Vec>(p, b, ch, valid, hist);
 }
 
 // Backward: p_t is computed again; dp_t = dy_t act'(p_t);  dx_t = sum_k w_k dp_{t+k};  dw_k = sum_t dp_t x_{t-k}.
@@ -187,9 +221,9 @@ __global__ void __launch_bounds__(128) conv_step_kernel(const __grid_constant__ 
 // as the rows before a sequence's start, and the final state's gradient joins the last W - 1 rows, which W - 1 more steps
 // with dp = 0 complete.  A strip also walks over the W - 1 tokens behind it, for its own last rows.
 template <int DT, int WT, bool Vec>
-__global__ void __launch_bounds__(32 * kBwdWarps) conv_bwd_kernel(const __grid_constant__ ConvP p) {
-    constexpr int PW = 4, U = 4;
-    __shared__ float red[kBwdWarps][WT + 1][32 * PW];
+__global__ void __launch_bounds__(32 * kBwdWarps, WT == 8 ? 1 : 2) conv_bwd_kernel(const __grid_constant__ ConvP p) {
+    constexpr int U = 4;
+    __shared__ __align__(16) float red[kBwdWarps][WT + 1][32 * PW];
     const int T = p.a.T, D = p.a.D, W = WT == 8 ? p.a.W : WT;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int cb = blockIdx.x % p.col_blocks, sb = blockIdx.x / p.col_blocks % p.strips, b = blockIdx.x / p.col_blocks / p.strips;
@@ -197,58 +231,86 @@ __global__ void __launch_bounds__(32 * kBwdWarps) conv_bwd_kernel(const __grid_c
     const long long first = ((long long)sb * kBwdWarps + warp) * p.strip;
     const Seqs q{p.a.cu_seqlens, p.a.cu_seqlens ? p.a.n_seqs : 1, T};
     const long long xrow = b * p.a.x_batch, yrow = (long long)b * T;
-    float w[WT][PW], bias[PW], dw[WT][PW] = {}, db[PW] = {}, xh[WT - 1][PW], dph[WT - 1][PW];
-    const float none[PW] = {};
+    const bool silu = p.a.activation == HDLA_ACT_SILU;
+    Quad dw[WT], db = {{0, 0}};
+#pragma unroll
+    for (int k = 0; k < WT; ++k) dw[k] = Quad{{0, 0}};
     if (valid > 0 && first < T) {
-        load_taps<PW, WT, Vec>(p, ch, valid, w, bias);
+        Quad w[WT], bias, xh[WT - 1], dph[WT - 1];
+        load_taps<WT, Vec>(p, ch, valid, w, bias);
         const int t0 = static_cast<int>(first), t1 = min(T, t0 + p.strip);
         int s = q.ends_behind(t0), start = 0, end = 0, from = 0;
-        // token t's dp (0 behind the sequence's end) completes row t - (W - 1)
-        auto emit = [&](int t, const float* dp) {
-            const int row = t - (W - 1);
-            float v[PW];
+        // what a token's dp (0 behind the sequence's end) completes: row t - (W - 1)
+        auto complete = [&](const Quad& dp) {
+            Quad v;
 #pragma unroll
-            for (int c = 0; c < PW; ++c) {
-                v[c] = 0.f;
+            for (int c = 0; c < 2; ++c) {
+                f2 r = 0;
 #pragma unroll
                 for (int k = 0; k < WT; ++k) {
-                    if (WT != 8) v[c] = fmaf(w[k][c], k == W - 1 ? dp[c] : dph[WT - 2 - k < 0 ? 0 : WT - 2 - k][c], v[c]);
+                    if (WT != 8) r = f2_fma(w[k].v[c], k == WT - 1 ? dp.v[c] : dph[WT - 2 - k < 0 ? 0 : WT - 2 - k].v[c], r);
                     else if (k < W) {
-                        float d = dp[c];
+                        f2 d = dp.v[c];
 #pragma unroll
                         for (int i = 0; i < WT - 1; ++i)
-                            if (i == W - 2 - k) d = dph[i][c];
-                        v[c] = fmaf(w[k][c], d, v[c]);
+                            if (i == W - 2 - k) d = dph[i].v[c];
+                        r = f2_fma(w[k].v[c], d, r);
                     }
                 }
+                v.v[c] = r;
             }
+            shift(dph, dp);
+            return v;
+        };
+        auto emit = [&](int t, const Quad& dp) {
+            const int row = t - (W - 1);
+            Quad v = complete(dp);
             if (t >= end && p.a.dht) {
-                float d[PW];
-                unpack<DT, PW>(ld_pack<DT, PW, Vec>(p.a.dht, ((long long)(b + s) * (W - 1) + (t - end)) * D + ch, valid), d);
-#pragma unroll
-                for (int c = 0; c < PW; ++c) v[c] += d[c];
+                const Quad d = quad_of<DT>(ld_pack<DT, PW, Vec>(p.a.dht, ((long long)(b + s) * (W - 1) + (t - end)) * D + ch, valid));
+                v.v[0] = f2_add(v.v[0], d.v[0]);
+                v.v[1] = f2_add(v.v[1], d.v[1]);
             }
             if (row >= from) {
-                if (row < t1) st_pack<DT, PW, Vec>(p.a.dx, (yrow + row) * D + ch, valid, v);
+                if (row < t1) st_quad<DT, Vec>(p.a.dx, (yrow + row) * D + ch, valid, v);
             } else if (from == start && p.a.dh0) {
-                st_pack<DT, PW, Vec>(p.a.dh0, ((long long)(b + s) * (W - 1) + (row - start + W - 1)) * D + ch, valid, v);
+                st_quad<DT, Vec>(p.a.dh0, ((long long)(b + s) * (W - 1) + (row - start + W - 1)) * D + ch, valid, v);
             }
-            shift<PW, WT - 1>(dph, dp);
+        };
+        // dp of a token, and its share of the weights' gradients where it is the strip's own
+        auto gradient = [&](const Pack<DT, PW>& xin, const Pack<DT, PW>& yin, bool mine) {
+            const Quad x = quad_of<DT>(xin);
+            Quad dp = quad_of<DT>(yin);
+            if (silu) {
+                const Quad pre = taps<WT>(w, bias, x, xh, W);
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {                  // silu' = s + p s (1 - s)
+                    const f2 sg = sigmoid_pair(pre.v[c]), ps = f2_mul(pre.v[c], sg);
+                    dp.v[c] = f2_mul(dp.v[c], f2_fma(ps, f2_fma(sg, f2_dup(-1.f), f2_dup(1.f)), sg));
+                }
+            }
+            if (mine)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    db.v[c] = f2_add(db.v[c], dp.v[c]);
+                    dw[0].v[c] = f2_fma(dp.v[c], x.v[c], dw[0].v[c]);
+#pragma unroll
+                    for (int k = 1; k < WT; ++k)
+                        if (WT != 8 || k < W) dw[k].v[c] = f2_fma(dp.v[c], xh[k - 1].v[c], dw[k].v[c]);
+                }
+            shift(xh, x);
+            return dp;
         };
         auto clear = [&] {
 #pragma unroll
-            for (int k = 0; k < WT - 1; ++k)
-#pragma unroll
-                for (int c = 0; c < PW; ++c) dph[k][c] = 0.f;
+            for (int k = 0; k < WT - 1; ++k) dph[k] = Quad{{0, 0}};
         };
+        const Quad none = {{0, 0}};
         auto empty = [&](int i, int at) {                      // an empty sequence at token `at`: dh0 = dht
             if (!p.a.dh0) return;
             const int keep = s;
             s = i; start = end = from = at;
             clear();
-            for (int f = 0; f < W - 1; ++f) {                  // its rows lie before `at`: nothing of dx is written
-                emit(at + f, none);
-            }
+            for (int f = 0; f < W - 1; ++f) emit(at + f, none);      // its rows lie before `at`: nothing of dx is written
             s = keep;
         };
         if (t0 == 0)
@@ -256,45 +318,31 @@ __global__ void __launch_bounds__(32 * kBwdWarps) conv_bwd_kernel(const __grid_c
         int t = t0;
         while (t < t1) {
             if (s >= q.n) {
-                for (; t < t1; ++t) st_pack<DT, PW, Vec>(p.a.dx, (yrow + t) * D + ch, valid, none);
+                for (; t < t1; ++t) st_quad<DT, Vec>(p.a.dx, (yrow + t) * D + ch, valid, none);
                 break;
             }
             start = min(q.off(s), t); end = max(q.off(s + 1), t); from = t;      // (offsets that decrease stay harmless)
             const int stop = min(end, t1 + W - 1);
-            load_hist<DT, PW, WT, Vec>(p, xrow, b + s, start, t, ch, valid, xh);
+            load_hist<DT, WT, Vec>(p, xrow, b + s, start, t, ch, valid, xh);
             clear();
             for (int tt = t; tt < stop; tt += U) {
                 Pack<DT, PW> xin[U], yin[U];
 #pragma unroll
-                for (int u = 0; u < U; ++u)
-                    if (tt + u < stop) {
-                        xin[u] = ld_pack<DT, PW, Vec>(p.a.x, xrow + (tt + u) * p.a.x_token + ch, valid);
-                        if (p.a.dy) yin[u] = ld_pack<DT, PW, Vec>(p.a.dy, (yrow + tt + u) * D + ch, valid);
-                        else yin[u] = {};
-                    }
-#pragma unroll
                 for (int u = 0; u < U; ++u) {
-                    if (tt + u >= stop) break;
-                    float x[PW], dp[PW], pre[PW];
-                    unpack<DT, PW>(xin[u], x);
-                    unpack<DT, PW>(yin[u], dp);
-                    if (p.a.activation == HDLA_ACT_SILU) {
-                        taps<PW, WT>(w, bias, x, xh, W, pre);
+                    const int ok = tt + u < stop ? valid : 0;
+                    xin[u] = ld_pack<DT, PW, Vec>(p.a.x, xrow + (tt + u) * p.a.x_token + ch, ok);
+                    yin[u] = ld_pack<DT, PW, Vec>(p.a.dy, (yrow + tt + u) * D + ch, p.a.dy ? ok : 0);
+                }
+                if (tt - (W - 1) >= from && tt + U <= min(stop, t1)) {       // rows and tokens of this strip and sequence
 #pragma unroll
-                        for (int c = 0; c < PW; ++c) dp[c] *= act_grad(pre[c], HDLA_ACT_SILU);
+                    for (int u = 0; u < U; ++u)
+                        st_quad<DT, Vec>(p.a.dx, (yrow + tt + u - (W - 1)) * D + ch, valid, complete(gradient(xin[u], yin[u], true)));
+                } else {
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        if (tt + u >= stop) break;
+                        emit(tt + u, gradient(xin[u], yin[u], tt + u < t1));
                     }
-                    if (tt + u < t1) {
-#pragma unroll
-                        for (int c = 0; c < PW; ++c) {
-                            db[c] += dp[c];
-                            dw[0][c] = fmaf(dp[c], x[c], dw[0][c]);
-#pragma unroll
-                            for (int k = 1; k < WT; ++k)
-                                if (WT != 8 || k < W) dw[k][c] = fmaf(dp[c], xh[k - 1][c], dw[k][c]);
-                        }
-                    }
-                    emit(tt + u, dp);
-                    shift<PW, WT - 1>(xh, x);
                 }
             }
             if (stop == end)
@@ -307,11 +355,8 @@ __global__ void __launch_bounds__(32 * kBwdWarps) conv_bwd_kernel(const __grid_c
         }
     }
 #pragma unroll
-    for (int k = 0; k < WT; ++k)
-#pragma unroll
-        for (int c = 0; c < PW; ++c) red[warp][k][lane * PW + c] = dw[k][c];
-#pragma unroll
-    for (int c = 0; c < PW; ++c) red[warp][WT][lane * PW + c] = db[c];
+    for (int k = 0; k < WT; ++k) *reinterpret_cast<ulonglong2*>(&red[warp][k][lane * PW]) = make_ulonglong2(dw[k].v[0], dw[k].v[1]);
+    *reinterpret_cast<ulonglong2*>(&red[warp][WT][lane * PW]) = make_ulonglong2(db.v[0], db.v[1]);
     __syncthreads();
     float* part = p.part + (long long)(b * p.strips + sb) * (W + 1) * D;
     for (int i = threadIdx.x; i < (W + 1) * 32 * PW; i += 32 * kBwdWarps) {
@@ -323,78 +368,68 @@ __global__ void __launch_bounds__(32 * kBwdWarps) conv_bwd_kernel(const __grid_c
     }
 }
 
-// Strips of 16 (forward) or 32 tokens (backward: also W - 1 tokens behind the strip) unless too few threads would be left to
-// keep the memory busy (about 512 an SM), then shorter ones.
-int strip_of(const HdlaConvArgs& a, int pw, int longest) {
-    int strip = longest;
-    while (strip > 4 && (long long)a.B * ((a.T + strip - 1) / strip) * ((a.D + pw - 1) / pw) < 512LL * sm_count()) strip /= 2;
-    return strip;
-}
-ConvP plan(const HdlaConvArgs& a, int pw, int longest, int warps) {
+// Strips of 32 tokens (backward also walks over W - 1 tokens behind the strip) unless too few threads would be left to keep the
+// memory busy (about 1024 an SM), then shorter ones.
+ConvP plan(const HdlaConvArgs& a, int warps) {
     ConvP p{};
     p.a = a;
-    p.strip = strip_of(a, pw, longest);
+    p.strip = 32;
+    while (p.strip > 4 && (long long)a.B * ((a.T + p.strip - 1) / p.strip) * ((a.D + PW - 1) / PW) < 1024LL * sm_count()) p.strip /= 2;
     p.strips = static_cast<int>(((long long)a.T + (long long)p.strip * warps - 1) / ((long long)p.strip * warps));
-    p.col_blocks = (a.D + 32 * pw - 1) / (32 * pw);
+    p.col_blocks = (a.D + 32 * PW - 1) / (32 * PW);
     p.wide_w = aligned16(a.weight);
     return p;
 }
-bool conv_vec(const HdlaConvArgs& a, int pw, int size) {
-    const int bytes = pw * size;
+bool conv_vec(const HdlaConvArgs& a) {
+    const int bytes = a.dtype == HDLA_F32 ? 16 : 8;
     auto ok = [&](const void* q) { return reinterpret_cast<uintptr_t>(q) % bytes == 0; };
-    return a.D % pw == 0 && a.x_batch % pw == 0 && a.x_token % pw == 0 && ok(a.x) && ok(a.h0) && ok(a.y) && ok(a.ht) && ok(a.dy) &&
+    return a.D % PW == 0 && a.x_batch % PW == 0 && a.x_token % PW == 0 && ok(a.x) && ok(a.h0) && ok(a.y) && ok(a.ht) && ok(a.dy) &&
            ok(a.dht) && ok(a.dx) && ok(a.dh0);
 }
 
-template <int DT, bool Vec, typename F>
+template <typename F>
 void with_taps(int W, F f) {
     if (W == 2) f(std::integral_constant<int, 2>());
     else if (W == 3) f(std::integral_constant<int, 3>());
     else if (W == 4) f(std::integral_constant<int, 4>());
     else f(std::integral_constant<int, 8>());
 }
+template <typename F>
+void with_type(int dtype, bool vec, F f) {
+    using F32 = std::integral_constant<int, HDLA_F32>;
+    using BF16 = std::integral_constant<int, HDLA_BF16>;
+    if (dtype == HDLA_F32) vec ? f(F32(), std::true_type()) : f(F32(), std::false_type());
+    else vec ? f(BF16(), std::true_type()) : f(BF16(), std::false_type());
+}
 
 }  // namespace
 
 int short_conv_fwd(const HdlaConvArgs& a, bool step, cudaStream_t st) {
-    const int size = a.dtype == HDLA_F32 ? 4 : 2, pw = 16 / size;
-    const bool vec = conv_vec(a, pw, size);
-    const ConvP p = plan(a, pw, 16, kFwdWarps);
+    const ConvP p = plan(a, kFwdWarps);
     const long long grid = step ? (long long)p.col_blocks * ((a.B + 3) / 4) : (long long)p.col_blocks * p.strips * a.B;
     if (grid > 0x7fffffffLL) return fail(HDLA_ERR_UNSUPPORTED, "short_conv: %lld blocks", grid);
-    auto go = [&](auto dt, auto v) {
-        with_taps<dt, v>(a.W, [&](auto wt) {
+    with_type(a.dtype, conv_vec(a), [&](auto dt, auto v) {
+        with_taps(a.W, [&](auto wt) {
             if (step) conv_step_kernel<dt, wt, v><<<(unsigned)grid, 128, 0, st>>>(p);
             else conv_fwd_kernel<dt, wt, v><<<(unsigned)grid, 32 * kFwdWarps, 0, st>>>(p);
         });
-    };
-    using F32 = std::integral_constant<int, HDLA_F32>;
-    using BF16 = std::integral_constant<int, HDLA_BF16>;
-    if (a.dtype == HDLA_F32) vec ? go(F32(), std::true_type()) : go(F32(), std::false_type());
-    else vec ? go(BF16(), std::true_type()) : go(BF16(), std::false_type());
+    });
     HDLA_CHECK_LAUNCH(step ? "conv_step_kernel" : "conv_fwd_kernel");
     return HDLA_OK;
 }
 
 size_t short_conv_bwd_workspace(const HdlaConvArgs& a) {
-    const ConvP p = plan(a, 4, 32, kBwdWarps);
-    return up256((size_t)a.B * p.strips * (a.W + 1) * a.D * sizeof(float));
+    return up256((size_t)a.B * plan(a, kBwdWarps).strips * (a.W + 1) * a.D * sizeof(float));
 }
 
 int short_conv_bwd(const HdlaConvArgs& a, float* part, cudaStream_t st) {
-    const int size = a.dtype == HDLA_F32 ? 4 : 2, pw = 4;
-    const bool vec = conv_vec(a, pw, size);
-    ConvP p = plan(a, pw, 32, kBwdWarps);
+    ConvP p = plan(a, kBwdWarps);
     p.part = part;
     const long long grid = (long long)p.col_blocks * p.strips * a.B;
     if (grid > 0x7fffffffLL) return fail(HDLA_ERR_UNSUPPORTED, "short_conv: %lld blocks", grid);
-    auto go = [&](auto dt, auto v) {
-        with_taps<dt, v>(a.W, [&](auto wt) { conv_bwd_kernel<dt, wt, v><<<(unsigned)grid, 32 * kBwdWarps, 0, st>>>(p); });
-    };
-    using F32 = std::integral_constant<int, HDLA_F32>;
-    using BF16 = std::integral_constant<int, HDLA_BF16>;
-    if (a.dtype == HDLA_F32) vec ? go(F32(), std::true_type()) : go(F32(), std::false_type());
-    else vec ? go(BF16(), std::true_type()) : go(BF16(), std::false_type());
+    with_type(a.dtype, conv_vec(a), [&](auto dt, auto v) {
+        with_taps(a.W, [&](auto wt) { conv_bwd_kernel<dt, wt, v><<<(unsigned)grid, 32 * kBwdWarps, 0, st>>>(p); });
+    });
     HDLA_CHECK_LAUNCH("conv_bwd_kernel");
     ColJobs js{};
     js.n = 1;
