@@ -10,7 +10,6 @@
 // the dot product of the pre norm's gradient; that of the post norm's), and keeps the sums over rows (gradients of the weights
 // and of scale) in registers until its last row; blocks' sums are added in a fixed order.  Rows of more than 4096 channels
 // need 1024 threads of 64 registers: there those sums are in shared memory too, and nothing is requested ahead.
-#include "f32x2.cuh"
 #include "ssm.cuh"
 
 namespace hdla {
@@ -25,7 +24,8 @@ struct NrP {
     float* part;             // backward: [blocks][3][D] (post, pre, scale)
 };
 
-// Sums over the warps of a row.  `red` has two buffers, used in turn, so that one barrier a sum is enough.
+// Sums over the warps of a row: over the lanes, then every warp over the warps' sums.  `red` has two buffers, used in turn, so
+// that one barrier a sum is enough.
 struct RowSum {
     float2 (*red)[32];
     int turn, first, warps;
@@ -33,26 +33,28 @@ struct RowSum {
 #pragma unroll
         for (int o = 16; o; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
         if (warps == 1) return a;
+        const int lane = threadIdx.x & 31;
         float* at = reinterpret_cast<float*>(red[turn]);
-        if ((threadIdx.x & 31) == 0) at[threadIdx.x >> 5] = a;
+        if (lane == 0) at[threadIdx.x >> 5] = a;
         __syncthreads();
-        float t = 0.f;
-#pragma unroll 4
-        for (int w = 0; w < warps; ++w) t += at[first + w];
+        a = lane < warps ? at[first + lane] : 0.f;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
         turn ^= 1;
-        return t;
+        return a;
     }
     __device__ __forceinline__ float2 two(float a, float b) {
         f2 v = f2_pack(a, b);
 #pragma unroll
         for (int o = 16; o; o >>= 1) v = f2_add(v, __shfl_xor_sync(0xffffffffu, v, o));
         if (warps > 1) {
+            const int lane = threadIdx.x & 31;
             f2* at = reinterpret_cast<f2*>(red[turn]);
-            if ((threadIdx.x & 31) == 0) at[threadIdx.x >> 5] = v;
+            if (lane == 0) at[threadIdx.x >> 5] = v;
             __syncthreads();
-            v = 0;
-#pragma unroll 4
-            for (int w = 0; w < warps; ++w) v = f2_add(v, at[first + w]);
+            v = lane < warps ? at[first + lane] : 0;
+#pragma unroll
+            for (int o = 16; o; o >>= 1) v = f2_add(v, __shfl_xor_sync(0xffffffffu, v, o));
             turn ^= 1;
         }
         float2 t;
@@ -117,11 +119,6 @@ struct GateAct {
         m = f2_dup(act == HDLA_ACT_SILU ? 1.f : 0.f);
         rest = f2_dup(act == HDLA_ACT_SILU ? 0.f : 1.f);
     }
-    __device__ __forceinline__ f2 sigmoid(f2 g) const {
-        float a, b;
-        f2_unpack(g, a, b);
-        return f2_pack(sigmoid_of(a), sigmoid_of(b));
-    }
     // from g and its sigmoid
     __device__ __forceinline__ f2 value(f2 g, f2 s) const { return plain ? g : f2_mul(s, f2_fma(g, m, rest)); }
     __device__ __forceinline__ f2 slope(f2 g, f2 s) const {
@@ -172,7 +169,7 @@ norm_residual_fwd_kernel(const __grid_constant__ NrP p) {
         }
         if (p.a.gate)
 #pragma unroll
-            for (int c = 0; c < kPairs; ++c) v[c] = f2_mul(v[c], act.value(g[c], act.sigmoid(g[c])));
+            for (int c = 0; c < kPairs; ++c) v[c] = f2_mul(v[c], act.value(g[c], sigmoid_pair(g[c])));
         ld_pairs(weights + 2 * p.stride + at.col, w);
         f2 ss = 0;
 #pragma unroll
@@ -261,7 +258,7 @@ __global__ void __launch_bounds__(MaxThreads, MaxThreads == 256 ? 2 : 1) norm_re
         if (p.a.gate) {
             unpack_pairs<DT>(cg, s);
 #pragma unroll
-            for (int c = 0; c < kPairs; ++c) s[c] = act.sigmoid(s[c]);
+            for (int c = 0; c < kPairs; ++c) s[c] = sigmoid_pair(s[c]);
         }
         unpack_pairs<RDT>(cd, d);
         if (p.a.pre_weight) {

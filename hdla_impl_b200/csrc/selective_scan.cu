@@ -215,55 +215,75 @@ __global__ void __launch_bounds__(kScanThreads, 5) scan_fwd_kernel(const __grid_
 
 // ------------------------------------------------------------------------------------------ single tokens
 // NL lanes a channel, four states a lane; a thread has the same channel in Rows sequences, so that A is read once and the
-// states' loads of Rows sequences are in flight together.  Bound by HBM: the fp32 state is read and written once.
+// states' loads of Rows sequences are in flight together.  What is done once per (sequence, channel) -- softplus, gate, the
+// loads and the store of x, dt, z, y -- each lane does for one of the sequences, and hands d and d x to the others of its
+// channel: done by every lane for every sequence it was three quarters of the instructions, and took longer than the memory.
+// Bound by HBM: the fp32 state is read and written once.
 template <int DT, int NL, int Rows>
 __global__ void __launch_bounds__(128) scan_step_kernel(const __grid_constant__ ScanP p) {
-    const int D = p.a.D, N = p.a.N, nl = threadIdx.x % NL, n0 = 4 * nl;
+    static_assert(Rows == 1 || Rows <= NL, "a lane has one of the sequences");
+    const int D = p.a.D, N = p.a.N, lane = threadIdx.x & 31, nl = lane % NL, n0 = 4 * nl;
     const int blocks = (D + 128 / NL - 1) / (128 / NL);
     const int d = blockIdx.x % blocks * (128 / NL) + threadIdx.x / NL, dd = min(d, D - 1), group = dd / p.Dg;
     const long long b0 = (long long)(blockIdx.x / blocks) * Rows;
+    const int rows = static_cast<int>(min((long long)Rows, p.a.B - b0));
     f2 A[2], h[Rows][2];
+    const float* state = p.a.h0 + ((size_t)b0 * D + dd) * N;
+    const size_t state_row = (size_t)D * N;
 #pragma unroll
     for (int r = 0; r < Rows; ++r)
-        if (b0 + r < p.a.B) ld_state(p.a.h0 + ((size_t)(b0 + r) * D + dd) * N, n0, N, p.vec_state, h[r]);
+        if (r < rows) ld_state(state + r * state_row, n0, N, p.vec_state, h[r]);
     ld_state(p.a.A + (size_t)dd * N, n0, N, p.vec_state, A);
-    const float bias = p.a.dt_bias ? p.a.dt_bias[dd] : 0.f, skip = p.a.skip ? p.a.skip[dd] : 0.f;
-    A[0] = f2_mul(A[0], f2_dup(kLog2e));
-    A[1] = f2_mul(A[1], f2_dup(kLog2e));
+    Pack<DT, 4> rB[Rows], rC[Rows];
+    const Walk fB = Walk::of<DT>(p.a.Bm, b0 * p.a.B_batch + group * p.a.B_group + n0, p.a.B_batch, 1);
+    const Walk fC = Walk::of<DT>(p.a.Cm, b0 * p.a.C_batch + group * p.a.C_group + n0, p.a.C_batch, 1);
 #pragma unroll
     for (int r = 0; r < Rows; ++r) {
-        const long long b = b0 + r;
-        if (b >= p.a.B) break;
-        float f[4], e;
+        const int valid = r < rows ? min(4, N - n0) : 0;
+        rB[r] = p.vec_bc ? fB.load<DT, true>(r, valid) : fB.load<DT, false>(r, valid);
+        rC[r] = p.vec_bc ? fC.load<DT, true>(r, valid) : fC.load<DT, false>(r, valid);
+    }
+    // this lane's sequence of the Rows
+    const int mine = scatter_at<Rows, NL>(lane, 1);
+    const long long b = b0 + min(mine, rows - 1);
+    const float x = ld_elem(p.a.x, b * p.a.x_batch + dd, DT), skip = p.a.skip ? p.a.skip[dd] : 0.f;
+    float dt = ld_elem(p.a.dt, b * p.a.dt_batch + dd, DT), z = 0.f;
+    if (p.a.z) z = ld_elem(p.a.z, b * p.a.z_batch + dd, DT);
+    if (p.a.dt_bias) dt += p.a.dt_bias[dd];
+    if (p.a.softplus) {
+        float unused;
+        f2_unpack(softplus_pair(f2_dup(dt)), dt, unused);
+    }
+    A[0] = f2_mul(A[0], f2_dup(kLog2e));
+    A[1] = f2_mul(A[1], f2_dup(kLog2e));
+    float y[Rows];
+#pragma unroll
+    for (int r = 0; r < Rows; ++r) {
+        int from = lane & ~(NL - 1);                           // the lane that has sequence r
+#pragma unroll
+        for (int l = 0; l < Rows; ++l)
+            if (scatter_at<Rows, NL>(l, 1) == r) from |= l;
+        const f2 d2 = f2_dup(Rows == 1 ? dt : __shfl_sync(0xffffffffu, dt, from));
+        const f2 u2 = f2_dup(Rows == 1 ? dt * x : __shfl_sync(0xffffffffu, dt * x, from));
         f2 B[2], C[2];
-        const long long ba = b * p.a.B_batch + group * p.a.B_group + n0, ca = b * p.a.C_batch + group * p.a.C_group + n0;
-        const int valid = min(4, N - n0);
-        unpack<DT, 4>(p.vec_bc ? ld_pack<DT, 4, true>(p.a.Bm, ba, valid) : ld_pack<DT, 4, false>(p.a.Bm, ba, valid), f);
-        B[0] = f2_pack(f[0], f[1]); B[1] = f2_pack(f[2], f[3]);
-        unpack<DT, 4>(p.vec_bc ? ld_pack<DT, 4, true>(p.a.Cm, ca, valid) : ld_pack<DT, 4, false>(p.a.Cm, ca, valid), f);
-        C[0] = f2_pack(f[0], f[1]); C[1] = f2_pack(f[2], f[3]);
-        const float x = ld_elem(p.a.x, b * p.a.x_batch + dd, DT);
-        float dt = ld_elem(p.a.dt, b * p.a.dt_batch + dd, DT) + bias;
-        if (p.a.softplus) dt = softplus_of(dt, e);
-        const f2 d2 = f2_dup(dt), u2 = f2_dup(dt * x);
+        unpack_pairs<DT>(rB[r], B);
+        unpack_pairs<DT>(rC[r], C);
 #pragma unroll
         for (int i = 0; i < 2; ++i) h[r][i] = f2_fma(ex2_pair(f2_mul(d2, A[i])), h[r][i], f2_mul(u2, B[i]));
-        float y = f2_sum(f2_fma(C[1], h[r][1], f2_mul(C[0], h[r][0])));
+        y[r] = f2_sum(f2_fma(C[1], h[r][1], f2_mul(C[0], h[r][0])));
+    }
+    scatter_sum<Rows, NL>(y, lane, 1);
+    if (d >= D) return;
+    float* to = p.a.ht + ((size_t)b0 * D + d) * N;
 #pragma unroll
-        for (int m = 1; m < NL; m <<= 1) y += __shfl_xor_sync(0xffffffffu, y, m);
-        y = fmaf(skip, x, y);
-        if (d >= D) continue;
-        st_state(p.a.ht + ((size_t)b * D + d) * N, n0, N, p.vec_state, h[r]);
-        if (nl == 0) {
-            if (p.a.z) {
-                const float z = ld_elem(p.a.z, b * p.a.z_batch + d, DT);
-                y *= z * sigmoid_of(z);
-            }
-            st_elem(p.a.y, b * D + d, DT, y);
-        }
+    for (int r = 0; r < Rows; ++r)
+        if (r < rows) st_state(to + r * state_row, n0, N, p.vec_state, h[r]);
+    if (nl < Rows && mine < rows) {
+        float v = fmaf(skip, x, y[0]);
+        if (p.a.z) v *= z * sigmoid_of(z);
+        st_elem(p.a.y, b * D + d, DT, v);
     }
 }
-
 
 int check_grid(long long blocks) {
     return blocks > 0x7fffffffLL ? fail(HDLA_ERR_UNSUPPORTED, "selective_scan: %lld blocks", blocks) : HDLA_OK;
@@ -376,14 +396,15 @@ int selective_scan_step(const HdlaScanArgs& a, cudaStream_t st) {
     const ScanP p = scan_params(a, r, ScanWork{}, nullptr);
     const int nl = scan_lanes(a.N);
     const long long columns = (a.D + 128 / nl - 1) / (128 / nl);
-    const bool many = columns * ((a.B + 3) / 4) >= 8LL * sm_count();       // four sequences a thread where enough blocks are left
-    const long long grid = columns * (many ? (a.B + 3) / 4 : a.B);
+    const int rows = nl == 2 ? 2 : 4;
+    const bool many = columns * ((a.B + rows - 1) / rows) >= 8LL * sm_count();     // several sequences a thread where enough blocks are left
+    const long long grid = columns * (many ? (a.B + rows - 1) / rows : a.B);
     if (int rc = check_grid(grid)) return rc;
     with_lanes(nl, [&](auto l) {
         using F32 = std::integral_constant<int, HDLA_F32>;
         using BF16 = std::integral_constant<int, HDLA_BF16>;
         auto go = [&](auto dt) {
-            if (many) scan_step_kernel<dt, l, 4><<<(unsigned)grid, 128, 0, st>>>(p);
+            if (many) scan_step_kernel<dt, l, l == 2 ? 2 : 4><<<(unsigned)grid, 128, 0, st>>>(p);
             else scan_step_kernel<dt, l, 1><<<(unsigned)grid, 128, 0, st>>>(p);
         };
         a.dtype == HDLA_F32 ? go(F32()) : go(BF16());

@@ -14,7 +14,6 @@
 // and F come from a first kernel that runs the recurrence alone, from zero; the second kernel's blocks chain the maps of
 // the segments before theirs.
 #pragma once
-#include "f32x2.cuh"
 #include "ssm.cuh"
 
 namespace hdla {
@@ -41,20 +40,6 @@ bool scan_vec(const HdlaScanArgs& a);              // four channels of every ten
 
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-
-__device__ __forceinline__ float ex2(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
-__device__ __forceinline__ float rcp(float x) { float r; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
-__device__ __forceinline__ f2 ex2_pair(f2 x) {
-    float a, b;
-    f2_unpack(x, a, b);
-    return f2_pack(ex2(a), ex2(b));
-}
-__device__ __forceinline__ f2 sigmoid_pair(f2 v) {
-    float a, b;
-    f2_unpack(f2_add(ex2_pair(f2_mul(v, f2_dup(-kLog2e))), f2_dup(1.f)), a, b);
-    return f2_pack(rcp(a), rcp(b));
-}
 // log(1 + e^v) = max(v, 0) + log1p(e), e = e^-|v| in (0, 1]; log1p(e) = 2 artanh(s) with s = e / (2 + e) <= 1/3, and artanh(s)
 // = s p(s^2), p the polynomial of degree 4 through the Chebyshev nodes of [0, 1/9], 4e-9 off at most.  (A logarithm of 1 + e
 // would lose the small time steps, which are e itself.)
@@ -70,8 +55,6 @@ __device__ __forceinline__ f2 softplus_pair(f2 v) {
     p = f2_fma(p, q, f2_dup(1.f));
     return f2_fma(f2_mul(s, p), f2_dup(2.f), f2_pack(fmaxf(a, 0.f), fmaxf(b, 0.f)));
 }
-// the derivative: 1 / (1 + e^-v)
-__device__ __forceinline__ f2 softplus_slope(f2 v) { return sigmoid_pair(v); }
 
 // four neighbouring channels as two pairs
 template <int DT>

@@ -336,7 +336,7 @@ __global__ void __launch_bounds__(kScanThreads, Maps ? 5 : 3) scan_bwd_kernel(co
                     }
                     dx[c] = f2_fma(d[c], dot[c], f2_mul(skip[c], g[c]));
                     dd[c] = f2_fma(x[c], dot[c], f2_mul(dec[c], f2_dup(kLn2)));      // (A is held times log2 e)
-                    if (p.a.softplus) dd[c] = f2_mul(dd[c], softplus_slope(f2_add(v[c], bias[c])));
+                    if (p.a.softplus) dd[c] = f2_mul(dd[c], sigmoid_pair(f2_add(v[c], bias[c])));
                     if (live < TB && tok >= live) dx[c] = dd[c] = dz[c] = 0;         // (g is zero)
                 }
                 {

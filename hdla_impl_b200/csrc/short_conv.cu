@@ -6,7 +6,6 @@
 // has just brought to L2.  Several tokens are requested at a time, and forward the next ones before these are worked on.  Four
 // channels a thread and not eight (16 bytes of bf16): the taps, their sums and the histories are what fills the registers, and
 // with half of them twice the warps hide the latency (forward 100 -> 57 us, backward 262 -> 128 us at 32768 x 2048, W = 4).
-#include "f32x2.cuh"
 #include "ssm.cuh"
 
 namespace hdla {
@@ -37,12 +36,6 @@ __device__ __forceinline__ void st_quad(void* base, long long i, int valid, cons
     f2_unpack(q.v[1], f[2], f[3]);
     st_pack<DT, PW, Vec>(base, i, valid, f);
 }
-__device__ __forceinline__ f2 sigmoid_pair(f2 v) {
-    float a, b;
-    f2_unpack(v, a, b);
-    return f2_pack(sigmoid_of(a), sigmoid_of(b));
-}
-
 // w[k]: the weights of lag k for the thread's channels
 template <int WT, bool Vec>
 __device__ __forceinline__ void load_taps(const ConvP& p, int ch, int valid, Quad (&w)[WT], Quad& bias) {
@@ -232,6 +225,8 @@ __global__ void __launch_bounds__(32 * kBwdWarps, WT == 8 ? 1 : 2) conv_bwd_kern
     const Seqs q{p.a.cu_seqlens, p.a.cu_seqlens ? p.a.n_seqs : 1, T};
     const long long xrow = b * p.a.x_batch, yrow = (long long)b * T;
     const bool silu = p.a.activation == HDLA_ACT_SILU;
+    constexpr int size = DT == HDLA_F32 ? 4 : 2;
+    const long long x_step = p.a.x_token * size, y_step = (long long)D * size;
     Quad dw[WT], db = {{0, 0}};
 #pragma unroll
     for (int k = 0; k < WT; ++k) dw[k] = Quad{{0, 0}};
@@ -325,25 +320,38 @@ __global__ void __launch_bounds__(32 * kBwdWarps, WT == 8 ? 1 : 2) conv_bwd_kern
             const int stop = min(end, t1 + W - 1);
             load_hist<DT, WT, Vec>(p, xrow, b + s, start, t, ch, valid, xh);
             clear();
+            const char* fx = static_cast<const char*>(p.a.x) + (xrow + t * p.a.x_token + ch) * size;
+            const char* fy = static_cast<const char*>(p.a.dy) + ((yrow + t) * D + ch) * size;
+            char* to = static_cast<char*>(p.a.dx) + ((yrow + t - (W - 1)) * D + ch) * size;
+            Pack<DT, PW> xn[U], yn[U];
+            auto request = [&](int tokens) {
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int ok = u < tokens ? valid : 0;
+                    xn[u] = ld_pack<DT, PW, Vec>(fx + u * x_step, 0, ok);
+                    yn[u] = ld_pack<DT, PW, Vec>(fy + u * y_step, 0, p.a.dy ? ok : 0);
+                }
+                fx += U * x_step;
+                fy += U * y_step;
+            };
+            request(stop - t);
             for (int tt = t; tt < stop; tt += U) {
                 Pack<DT, PW> xin[U], yin[U];
 #pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const int ok = tt + u < stop ? valid : 0;
-                    xin[u] = ld_pack<DT, PW, Vec>(p.a.x, xrow + (tt + u) * p.a.x_token + ch, ok);
-                    yin[u] = ld_pack<DT, PW, Vec>(p.a.dy, (yrow + tt + u) * D + ch, p.a.dy ? ok : 0);
-                }
+                for (int u = 0; u < U; ++u) { xin[u] = xn[u]; yin[u] = yn[u]; }
+                if (tt + U < stop) request(stop - tt - U);
                 if (tt - (W - 1) >= from && tt + U <= min(stop, t1)) {       // rows and tokens of this strip and sequence
 #pragma unroll
-                    for (int u = 0; u < U; ++u)
-                        st_quad<DT, Vec>(p.a.dx, (yrow + tt + u - (W - 1)) * D + ch, valid, complete(gradient(xin[u], yin[u], true)));
+                    for (int u = 0; u < U; ++u) st_quad<DT, Vec>(to + u * y_step, 0, valid, complete(gradient(xin[u], yin[u], true)));
                 } else {
+#pragma unroll 1
+                    for (int u = 0; u < min(U, stop - tt); ++u) {
+                        emit(tt + u, gradient(xin[0], yin[0], tt + u < t1));
 #pragma unroll
-                    for (int u = 0; u < U; ++u) {
-                        if (tt + u >= stop) break;
-                        emit(tt + u, gradient(xin[u], yin[u], tt + u < t1));
+                        for (int i = 0; i < U - 1; ++i) { xin[i] = xin[i + 1]; yin[i] = yin[i + 1]; }
                     }
                 }
+                to += U * y_step;
             }
             if (stop == end)
                 for (int f = 0; f < W - 1; ++f) emit(end + f, none);

@@ -2,6 +2,7 @@
 // moved as one access, activations, and sums over partial rows in a fixed order.
 #pragma once
 #include "common.cuh"
+#include "f32x2.cuh"
 
 namespace hdla {
 namespace {
@@ -137,30 +138,20 @@ __device__ __forceinline__ void st_pack(void* base, long long i, int valid, cons
 }
 
 // ------------------------------------------------------------------------------------------ activations
-__device__ __forceinline__ float sigmoid_of(float v) { return __fdividef(1.f, 1.f + __expf(-v)); }   // (e^-v = inf: 0)
-__device__ __forceinline__ float act_of(float v, int act) {
-    return act == HDLA_ACT_SILU ? v * sigmoid_of(v) : act == HDLA_ACT_SIGMOID ? sigmoid_of(v) : v;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+__device__ __forceinline__ float ex2(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
+__device__ __forceinline__ float rcp(float x) { float r; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
+__device__ __forceinline__ f2 ex2_pair(f2 x) {
+    float a, b;
+    f2_unpack(x, a, b);
+    return f2_pack(ex2(a), ex2(b));
 }
-__device__ __forceinline__ float act_grad(float v, int act) {
-    if (act == HDLA_ACT_NONE) return 1.f;
-    const float s = sigmoid_of(v);
-    return act == HDLA_ACT_SILU ? s * (1.f + v * (1.f - s)) : s * (1.f - s);
+__device__ __forceinline__ float sigmoid_of(float v) { return rcp(1.f + ex2(-kLog2e * v)); }           // (e^-v = inf: 0)
+__device__ __forceinline__ f2 sigmoid_pair(f2 v) {
+    float a, b;
+    f2_unpack(f2_add(ex2_pair(f2_mul(v, f2_dup(-kLog2e))), f2_dup(1.f)), a, b);
+    return f2_pack(rcp(a), rcp(b));
 }
-// log(1 + e^v) = max(v, 0) + log1p(e), e = e^-|v| in (0, 1]: log1p(e) = 2 artanh(s), s = e / (2 + e) <= 1/3, by the series
-// s + s^3/3 + ... + s^13/13, whose remainder at s = 1/3 is 1.6e-8 of the sum.  (A logarithm of 1 + e would lose the
-// small time steps: they are e itself.)  `e` is handed back for the derivative.
-__device__ __forceinline__ float softplus_of(float v, float& e) {
-    e = __expf(-fabsf(v));
-    const float s = __fdividef(e, 2.f + e), q = s * s;
-    float p = fmaf(q, 1.f / 13.f, 1.f / 11.f);
-    p = fmaf(p, q, 1.f / 9.f);
-    p = fmaf(p, q, 1.f / 7.f);
-    p = fmaf(p, q, 1.f / 5.f);
-    p = fmaf(p, q, 1.f / 3.f);
-    p = fmaf(p, q, 1.f);
-    return fmaxf(v, 0.f) + 2.f * s * p;
-}
-
 // ------------------------------------------------------------------------------------------ sums over partial rows
 // out[c] = sum over P rows of part[row, c], in the rows' order by eight- and sixteenfold strides that depend on P alone.
 // Column c = (r * K + k) * NP + n goes to out[k][r * N + n] where n < N; with `turned` column n * K + k of a [NP, K] matrix
