@@ -13,7 +13,7 @@ template <int DT, bool Vec, int NL, int CT, bool Maps>
 __global__ void __launch_bounds__(kScanThreads, 5) scan_fwd_kernel(const __grid_constant__ ScanP p) {
     using TileT = Tile<NL, CT>;
     constexpr int NP = TileT::NP, CH = TileT::CH, Pitch = TileT::Pitch, PW = 4;
-    constexpr int TB = CH >= 64 || NL >= 16 ? 8 : 16, Groups = CH / PW, Items = TB * Groups, IT = (Items + kScanThreads - 1) / kScanThreads;
+    constexpr int TB = CH > 64 || NL >= 16 ? 8 : 16, Groups = CH / PW, Items = TB * Groups, IT = (Items + kScanThreads - 1) / kScanThreads;
     static_assert(CH % PW == 0 && kScanThreads % Groups == 0, "a thread's pieces are of one group of channels");
     __shared__ __align__(16) float s_d[TB][CH], s_u[TB][CH], s_B[TB][NP], s_C[TB][NP], s_y[Maps ? 1 : TB * NL][Pitch];
 
@@ -298,12 +298,14 @@ int scan_lanes(int N) {
     return nl;
 }
 
-// Channels a lane, and segments.  Four blocks an SM hide the latencies of the forward kernel, three those of the backward one;
-// two channels a lane are cheaper in shared-memory cycles than one, one channel a lane gives twice the blocks.  Cutting rows
-// runs the recurrence once more for the maps, and pays only where too few blocks would be left.  Measured at N = 16, 8 x 2048
-// channels, T = 4096, forward: one channel, whole rows (512 blocks) 606 us; two channels, whole rows (256 blocks) 729 us; two
-// channels, 16 segments 439 + 288 us for the maps.  Backward (two channels): whole rows 2070 us, 8 segments 1485 + 368 us.  One row of 2048 channels, T = 65536, forward: 32 segments
-// 1527 us, 64 segments 1459 us.  So rows are cut into segments of 64 tokens or more until there are twelve blocks an SM.
+// Channels a lane, and segments.  Five blocks an SM are resident forward, three backward, and about so many hide the latencies.
+// Two channels a lane are cheaper in shared-memory cycles than one, one channel a lane gives twice the blocks.  Cutting rows
+// runs the recurrence once more for the maps, and pays only where too few blocks would be left.  Measured at N = 16, 8 rows of
+// 2048 channels, T = 4096.  Forward: one channel, whole rows (512 blocks) 600 us; two channels, whole rows (256 blocks) 729 us;
+// two channels, 16 segments 434 + 286 us for the maps.  Backward (two channels): whole rows 2070 us, 7 segments (4.04 rounds of
+// resident blocks) 1584 + 365 us, 8 segments (4.6 rounds) 1485 + 368 us, 12 segments 1489 + 365 us.  One row of 2048
+// channels, T = 65536, forward: 32 segments 1527 us, 64 segments 1443 us.  So rows are cut into segments of 64 tokens or more
+// until there are thirteen blocks an SM.
 ScanPlan scan_plan(const HdlaScanArgs& a, bool backward) {
     const int nl = scan_lanes(a.N), dg = a.D / a.G, sms = sm_count();
     ScanPlan r{};
@@ -316,10 +318,10 @@ ScanPlan scan_plan(const HdlaScanArgs& a, bool backward) {
     long long n, cut = 1;
     if (backward) {
         n = blocks(nl == 2 || nl == 32 ? 1 : 2);
-        if (n < 2.5 * sms) cut = (12LL * sms + n - 1) / n;
+        if (n < 2.5 * sms) cut = (13LL * sms + n - 1) / n;
     } else if ((n = blocks(2)) < 3.5 * sms && (n = blocks(1)) < 2LL * sms) {
         n = blocks(2);
-        cut = (12LL * sms + n - 1) / n;
+        cut = (13LL * sms + n - 1) / n;
     }
     const long long most = (a.T + 63) / 64;
     if (cut > most) cut = most;
