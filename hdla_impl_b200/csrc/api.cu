@@ -345,7 +345,8 @@ size_t hdla_norm_residual_bwd_workspace_bytes(const HdlaNormResidualArgs* args) 
 
 int hdla_norm_residual_bwd(const HdlaNormResidualArgs* args, void* workspace, size_t workspace_bytes, void* cuda_stream) {
     if (int rc = check_norm(args)) return rc;
-    if (!args->x || !args->dx) return fail(HDLA_ERR_INVALID, "norm_residual_bwd: null tensor pointer");
+    if (!args->x || !args->dx || ((args->post_weight || args->pre_weight) && !args->factors))
+        return fail(HDLA_ERR_INVALID, "norm_residual_bwd: null tensor pointer");
     if (int rc = check_space("norm_residual_bwd", norm_residual_bwd_workspace(*args), workspace, workspace_bytes)) return rc;
     begin_call(static_cast<cudaStream_t>(cuda_stream));
     return norm_residual_bwd(*args, static_cast<float*>(workspace), static_cast<cudaStream_t>(cuda_stream));

@@ -449,17 +449,20 @@ HdlaNormResidualArgs norm_args(const NormIn& i) {
     a.x = ptr(i.x); a.residual = ptr(i.r); a.gate = ptr(i.g); a.post_weight = ptr(i.post); a.pre_weight = ptr(i.pre); a.scale = ptr(i.scale);
     return a;
 }
-std::pair<Tensor, Tensor> norm_forward(const NormIn& i) {
+struct NormOut { Tensor r, u, factors; };
+NormOut norm_forward(const NormIn& i, bool keep) {
     HdlaNormResidualArgs a = norm_args(i);
     const Tensor r = dense(i.x.sizes(), i.r.defined() ? i.r.scalar_type() : i.x.scalar_type(), i.x.device());
     Tensor u;
     if (i.pre.defined()) u = dense_like(i.x);
-    a.r = mptr(r); a.u = mptr(u);
+    Tensor factors;
+    if (keep && (i.post.defined() || i.pre.defined())) factors = dense({a.rows, 2}, at::kFloat, i.x.device());
+    a.r = mptr(r); a.u = mptr(u); a.factors = fptr(factors);
     check(ssm.norm_fwd(&a, stream_of(i.x)), "hdla_norm_residual_fwd");
-    return {r, u};
+    return {r, u, factors};
 }
 struct NormGrads { Tensor dx, dr, dg, dpost, dpre, dscale; };
-NormGrads norm_backward(const NormIn& i, const Tensor& dr_, const Tensor& du_) {
+NormGrads norm_backward(const NormIn& i, const Tensor& factors, const Tensor& dr_, const Tensor& du_) {
     c10::cuda::CUDAGuard guard(i.x.device());
     HdlaNormResidualArgs a = norm_args(i);
     const Tensor dr = grad_in(dr_, i.r.defined() ? i.r.scalar_type() : i.x.scalar_type()), du = grad_in(du_, i.x.scalar_type());
@@ -467,7 +470,7 @@ NormGrads norm_backward(const NormIn& i, const Tensor& dr_, const Tensor& du_) {
     NormGrads g{like(i.x), like(i.r), like(i.g), like(i.post), like(i.pre), like(i.scale)};
     const size_t n = ssm.norm_bwd_bytes(&a);
     const Tensor ws = space(n, i.x);
-    a.dr = ptr(dr); a.du = ptr(du);
+    a.dr = ptr(dr); a.du = ptr(du); a.factors = fptr(factors);
     a.dx = mptr(g.dx); a.dresidual = mptr(g.dr); a.dgate = mptr(g.dg);
     a.dpost_weight = mptr(g.dpost); a.dpre_weight = mptr(g.dpre); a.dscale = mptr(g.dscale);
     check(ssm.norm_bwd(&a, mptr(ws), n, stream_of(i.x)), "hdla_norm_residual_bwd");
@@ -490,12 +493,14 @@ NormIn norm_in(const NormCall& c) {
 
 struct NormResidualNode : torch::autograd::Node {
     Saved x, r, g, post, pre, scale;
+    Tensor factors;                                  // read only
     NormIn rest;                                     // the numbers; no tensors
     at::ScalarType post_type = at::kFloat, pre_type = at::kFloat, scale_type = at::kFloat;
     std::string name() const override { return "HdlaNormResidualBackward"; }
     void release_variables() override {
         std::lock_guard<std::mutex> lock(mutex_);
         for (Saved* s : {&x, &r, &g, &post, &pre, &scale}) s->var.reset_data();
+        factors = Tensor();
     }
     variable_list apply(variable_list&& grads) override {
         std::lock_guard<std::mutex> lock(mutex_);
@@ -505,23 +510,24 @@ struct NormResidualNode : torch::autograd::Node {
         const char* me = "HdlaNormResidualBackward";
         NormIn i = rest;
         i.x = x.get(me); i.r = r.get(me); i.g = g.get(me); i.post = post.get(me); i.pre = pre.get(me); i.scale = scale.get(me);
-        NormGrads d = norm_backward(i, grads[0], du);
+        NormGrads d = norm_backward(i, factors, grads[0], du);
         return {d.dx, d.dr, d.dg, as_type(d.dscale, scale_type), as_type(d.dpost, post_type), as_type(d.dpre, pre_type)};
     }
 };
 
 std::pair<Tensor, Tensor> norm_residual_op(const NormCall& c) {
     const bool grad = needs_grad({c.x, c.r, c.g, c.scale, c.post, c.pre});
-    std::pair<Tensor, Tensor> out;
+    NormOut out;
     std::shared_ptr<NormResidualNode> node;
     {
         at::NoGradGuard no_grad;
         c10::cuda::CUDAGuard guard(c.x->device());
         const NormIn i = norm_in(c);
-        out = norm_forward(i);
+        out = norm_forward(i, grad);
         if (grad) {
             node = make_node<NormResidualNode>();
             node->x.save(i.x); node->r.save(i.r); node->g.save(i.g); node->post.save(i.post); node->pre.save(i.pre); node->scale.save(i.scale);
+            node->factors = out.factors;
             node->rest.scale_value = i.scale_value; node->rest.eps = i.eps; node->rest.act = i.act; node->rest.w_type = i.w_type;
             if (c.post->defined()) node->post_type = c.post->scalar_type();
             if (c.pre->defined()) node->pre_type = c.pre->scalar_type();
@@ -530,10 +536,10 @@ std::pair<Tensor, Tensor> norm_residual_op(const NormCall& c) {
     }
     if (grad) {
         node->set_next_edges(torch::autograd::collect_next_edges(*c.x, *c.r, *c.g, *c.scale, *c.post, *c.pre));
-        torch::autograd::create_gradient_edge(out.first, node);
-        if (out.second.defined()) torch::autograd::create_gradient_edge(out.second, node);
+        torch::autograd::create_gradient_edge(out.r, node);
+        if (out.u.defined()) torch::autograd::create_gradient_edge(out.u, node);
     }
-    return out;
+    return {out.r, out.u};
 }
 
 // (x, residual or None, gate or None, scale: a vector or a number, post or None, pre or None, activation code, eps) at av
@@ -557,28 +563,40 @@ bool norm_call(PyObject* const* av, NormCall& c) {
     return same_device(x, {c.r, c.g, c.scale, c.post, c.pre});
 }
 
-// norm_residual(...) -> (r, u or None)
+// norm_residual(..., keep or None): keep None: the differentiable operator, (r, u or None); True or False: a bare forward call,
+// (r, u or None, the norms' factors or None)
 PyObject* py_norm_residual(PyObject*, PyObject* const* av, Py_ssize_t n) {
-    if (n != 8) { PyErr_SetString(PyExc_TypeError, "norm_residual takes 8 arguments"); return nullptr; }
+    if (n != 9) { PyErr_SetString(PyExc_TypeError, "norm_residual takes 9 arguments"); return nullptr; }
     NormCall c;
-    if (tracing() || !norm_call(av, c)) NOT_MINE();
-    std::pair<Tensor, Tensor> r;
-    if (!guarded([&] { r = norm_residual_op(c); })) return nullptr;
-    return tuple_of({&r.first, &r.second});
+    const bool bare = av[8] != Py_None;
+    if ((!bare && tracing()) || !norm_call(av, c)) NOT_MINE();
+    NormOut r;
+    if (!guarded([&] {
+            if (bare) {
+                at::NoGradGuard no_grad;
+                c10::cuda::CUDAGuard guard(c.x->device());
+                r = norm_forward(norm_in(c), av[8] == Py_True);
+            } else {
+                std::tie(r.r, r.u) = norm_residual_op(c);
+            }
+        }))
+        return nullptr;
+    return bare ? tuple_of({&r.r, &r.u, &r.factors}) : tuple_of({&r.r, &r.u});
 }
-// norm_residual_backward(..., dr or None, du or None) -> gradients of (x, residual, gate, scale, post, pre)
+// norm_residual_backward(..., factors or None, dr or None, du or None) -> gradients of (x, residual, gate, scale, post, pre)
 PyObject* py_norm_residual_backward(PyObject*, PyObject* const* av, Py_ssize_t n) {
-    if (n != 10) { PyErr_SetString(PyExc_TypeError, "norm_residual_backward takes 10 arguments"); return nullptr; }
+    if (n != 11) { PyErr_SetString(PyExc_TypeError, "norm_residual_backward takes 11 arguments"); return nullptr; }
     NormCall c;
-    const Tensor *dr = arg(av[8], true), *du = arg(av[9], true);
-    if (!norm_call(av, c) || !dr || !du) {
+    const Tensor *factors = arg(av[8], true), *dr = arg(av[9], true), *du = arg(av[10], true);
+    if (!norm_call(av, c) || !factors || !dr || !du ||
+        (factors->defined() && (factors->scalar_type() != at::kFloat || !factors->is_contiguous() || factors->numel() != 2 * (c.x->numel() / c.x->size(-1))))) {
         PyErr_SetString(PyExc_TypeError, "norm_residual_backward: arguments of another kind than the forward call's");
         return nullptr;
     }
     NormGrads g;
     if (!guarded([&] {
             at::NoGradGuard no_grad;
-            g = norm_backward(norm_in(c), *dr, *du);
+            g = norm_backward(norm_in(c), *factors, *dr, *du);
             if (g.dscale.defined()) g.dscale = as_type(g.dscale, c.scale->scalar_type());
             if (g.dpost.defined()) g.dpost = as_type(g.dpost, c.post->scalar_type());
             if (g.dpre.defined()) g.dpre = as_type(g.dpre, c.pre->scalar_type());

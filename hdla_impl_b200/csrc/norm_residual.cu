@@ -6,8 +6,8 @@
 // sums; a row takes as many whole warps as it needs, narrow rows share a block.  Blocks walk over rows and request the next
 // row's tensors before the sums of this one; the weights wait in shared memory, so that two (backward) or four (forward) blocks
 // of 256 threads fit on an SM: with them in registers backward had one, and took 686 instead of 300 us for 32768 rows of 2048.
-// Backward computes r again from the inputs in fp32 (as many bytes as reading the rounded r), takes three sums (x^2; r^2 with
-// the dot product of the pre norm's gradient; that of the post norm's), and keeps the sums over rows (gradients of the weights
+// Backward computes r again from the inputs in fp32 (as many bytes as reading the rounded r), reads the norms' factors that
+// forward left, takes the two sums that remain (the dot products of the norms' gradients), and keeps the sums over rows (gradients of the weights
 // and of scale) in registers until its last row; blocks' sums are added in a fixed order.  Rows of more than 4096 channels
 // need 1024 threads of 64 registers: there those sums are in shared memory too, and nothing is requested ahead.
 #include "ssm.cuh"
@@ -27,39 +27,25 @@ struct NrP {
 // Sums over the warps of a row: over the lanes, then every warp over the warps' sums.  `red` has two buffers, used in turn, so
 // that one barrier a sum is enough.
 struct RowSum {
-    float2 (*red)[32];
+    float (*red)[32];
     int turn, first, warps;
     __device__ __forceinline__ float one(float a) {
 #pragma unroll
         for (int o = 16; o; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
         if (warps == 1) return a;
-        const int lane = threadIdx.x & 31;
-        float* at = reinterpret_cast<float*>(red[turn]);
-        if (lane == 0) at[threadIdx.x >> 5] = a;
+        float* at = red[turn];
+        if ((threadIdx.x & 31) == 0) at[threadIdx.x >> 5] = a;
         __syncthreads();
-        a = lane < warps ? at[first + lane] : 0.f;
+        const int w = threadIdx.x & (warps > 8 ? 31 : 7);
+        a = w < warps ? at[first + w] : 0.f;
+        if (warps > 8) {
+            a += __shfl_xor_sync(0xffffffffu, a, 16);
+            a += __shfl_xor_sync(0xffffffffu, a, 8);
+        }
 #pragma unroll
-        for (int o = 16; o; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+        for (int o = 4; o; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
         turn ^= 1;
         return a;
-    }
-    __device__ __forceinline__ float2 two(float a, float b) {
-        f2 v = f2_pack(a, b);
-#pragma unroll
-        for (int o = 16; o; o >>= 1) v = f2_add(v, __shfl_xor_sync(0xffffffffu, v, o));
-        if (warps > 1) {
-            const int lane = threadIdx.x & 31;
-            f2* at = reinterpret_cast<f2*>(red[turn]);
-            if (lane == 0) at[threadIdx.x >> 5] = v;
-            __syncthreads();
-            v = lane < warps ? at[first + lane] : 0;
-#pragma unroll
-            for (int o = 16; o; o >>= 1) v = f2_add(v, __shfl_xor_sync(0xffffffffu, v, o));
-            turn ^= 1;
-        }
-        float2 t;
-        f2_unpack(v, t.x, t.y);
-        return t;
     }
 };
 
@@ -130,7 +116,7 @@ template <int DT, int RDT, bool Vec, int MaxThreads>
 __global__ void __launch_bounds__(MaxThreads, MaxThreads == 256 ? 4 : MaxThreads == 512 ? 2 : 1)
 norm_residual_fwd_kernel(const __grid_constant__ NrP p) {
     extern __shared__ __align__(16) float weights[];
-    __shared__ float2 red[2][32];
+    __shared__ float red[2][32];
     put_weights(p, weights);
     const Place at(p);
     const int D = p.a.D;
@@ -138,10 +124,11 @@ norm_residual_fwd_kernel(const __grid_constant__ NrP p) {
     const GateAct act(p.a.activation);
     const float root = sqrtf((float)D);
     constexpr bool Ahead = MaxThreads <= 512;
-    Pack<DT, kPw> nx, ng = {};
+    Pack<DT, kPw> nx = {}, ng = {};
     Pack<RDT, kPw> nr = {};
     auto request = [&](long long row) {
         const int ok = row < p.a.rows ? at.valid : 0;
+        if (ok <= 0 && at.rows == 1) return;                // (a thread behind the row's end keeps its zeros)
         const long long i = row * D + at.col;
         nx = ld_pack<DT, kPw, Vec>(p.a.x, i, ok);
         if (p.a.residual) nr = ld_pack<RDT, kPw, Vec>(p.a.residual, i, ok);
@@ -157,12 +144,14 @@ norm_residual_fwd_kernel(const __grid_constant__ NrP p) {
         unpack_pairs<DT>(nx, v);
         unpack_pairs<DT>(ng, g);
         unpack_pairs<RDT>(nr, r);
-        if (Ahead) request(row + step);
+        if (Ahead && first + step < p.a.rows) request(row + step);
         if (p.a.post_weight) {
             f2 ss = 0;
 #pragma unroll
             for (int c = 0; c < kPairs; ++c) ss = f2_fma(v[c], v[c], ss);
-            const f2 k = f2_dup(root * rsqrtf(sum.one(f2_sum(ss)) + p.a.eps));
+            const float factor = root * rsqrtf(sum.one(f2_sum(ss)) + p.a.eps);
+            if (p.a.factors && at.col == 0 && row < p.a.rows) p.a.factors[2 * row] = factor;
+            const f2 k = f2_dup(factor);
             ld_pairs(weights + at.col, w);
 #pragma unroll
             for (int c = 0; c < kPairs; ++c) v[c] = f2_mul(v[c], f2_mul(k, w[c]));
@@ -180,7 +169,9 @@ norm_residual_fwd_kernel(const __grid_constant__ NrP p) {
         const int ok = row < p.a.rows ? at.valid : 0;
         st_row<RDT, Vec>(p.a.r, row * D + at.col, ok, r);
         if (p.a.pre_weight) {
-            const f2 k = f2_dup(root * rsqrtf(sum.one(f2_sum(ss)) + p.a.eps));
+            const float factor = root * rsqrtf(sum.one(f2_sum(ss)) + p.a.eps);
+            if (p.a.factors && at.col == 0 && row < p.a.rows) p.a.factors[2 * row + 1] = factor;
+            const f2 k = f2_dup(factor);
             ld_pairs(weights + p.stride + at.col, w);
 #pragma unroll
             for (int c = 0; c < kPairs; ++c) r[c] = f2_mul(r[c], f2_mul(k, w[c]));
@@ -192,7 +183,7 @@ norm_residual_fwd_kernel(const __grid_constant__ NrP p) {
 template <int DT, int RDT, bool Vec, int MaxThreads>
 __global__ void __launch_bounds__(MaxThreads, MaxThreads == 256 ? 2 : 1) norm_residual_bwd_kernel(const __grid_constant__ NrP p) {
     extern __shared__ __align__(16) float weights[];        // 3 vectors; 3 of sums behind them where those are not in registers
-    __shared__ float2 red[2][32];
+    __shared__ float red[2][32];
     constexpr bool Lean = MaxThreads > 512;
     put_weights(p, weights);
     const Place at(p);
@@ -222,11 +213,18 @@ __global__ void __launch_bounds__(MaxThreads, MaxThreads == 256 ? 2 : 1) norm_re
             for (int c = 0; c < kPairs; ++c) acc[k][c] = f2_fma(a[c], b[c], acc[k][c]);
         }
     };
-    const float root = sqrtf((float)D), per = 1.f / (float)D;
-    Pack<DT, kPw> nx, ng = {}, nu = {};
+    const float per = 1.f / (float)D;
+    float fx = 0.f, fr = 0.f;                               // the norms' factors of the next row
+    auto factors = [&](long long row) {
+        if (row >= p.a.rows) return;
+        if (p.a.post_weight) fx = __ldg(p.a.factors + 2 * row);
+        if (p.a.pre_weight) fr = __ldg(p.a.factors + 2 * row + 1);
+    };
+    Pack<DT, kPw> nx = {}, ng = {}, nu = {};
     Pack<RDT, kPw> nr = {}, nd = {};
     auto request = [&](long long row) {
         const int ok = row < p.a.rows ? at.valid : 0;
+        if (ok <= 0 && at.rows == 1) return;                // (a thread behind the row's end keeps its zeros)
         const long long i = row * D + at.col;
         nx = ld_pack<DT, kPw, Vec>(p.a.x, i, ok);
         if (p.a.residual) nr = ld_pack<RDT, kPw, Vec>(p.a.residual, i, ok);
@@ -237,24 +235,19 @@ __global__ void __launch_bounds__(MaxThreads, MaxThreads == 256 ? 2 : 1) norm_re
     long long first = (long long)blockIdx.x * at.rows;
     const long long step = (long long)gridDim.x * at.rows;
     if (!Lean) request(first + at.group);
+    factors(first + at.group);
     for (; first < p.a.rows; first += step) {
         const long long row = first + at.group;
         if (Lean) request(row);
         const Pack<DT, kPw> cx = nx, cg = ng, cu = nu;
         const Pack<RDT, kPw> cr = nr, cd = nd;
-        if (!Lean) request(row + step);
+        if (!Lean && first + step < p.a.rows) request(row + step);
         const bool exists = row < p.a.rows;                 // (a block's last rows may not)
         // what is used twice is unpacked twice: registers are short
         f2 s[kPairs], d[kPairs];                            // the gate's sigmoid; the gradient on its way from r to x
-        float kx = 1.f;                                     // n = x kx post, v = n act(g), r = residual + scale v
-        if (p.a.post_weight) {
-            f2 x[kPairs], ss = 0;
-            unpack_pairs<DT>(cx, x);
-#pragma unroll
-            for (int c = 0; c < kPairs; ++c) ss = f2_fma(x[c], x[c], ss);
-            const float t = sum.one(f2_sum(ss));
-            kx = exists ? root * rsqrtf(t + p.a.eps) : 0.f;
-        }
+        // n = x kx post, v = n act(g), r = residual + scale v
+        const float kx = !p.a.post_weight ? 1.f : exists ? fx : 0.f, kr = exists ? fr : 0.f;
+        if (first + step < p.a.rows) factors(row + step);
         if (p.a.gate) {
             unpack_pairs<DT>(cg, s);
 #pragma unroll
@@ -262,7 +255,7 @@ __global__ void __launch_bounds__(MaxThreads, MaxThreads == 256 ? 2 : 1) norm_re
         }
         unpack_pairs<RDT>(cd, d);
         if (p.a.pre_weight) {
-            f2 x[kPairs], r[kPairs], w[kPairs], k[kPairs], ss = 0, dot = 0;
+            f2 x[kPairs], r[kPairs], w[kPairs], k[kPairs], dot = 0;
             unpack_pairs<DT>(cx, x);
             ld_pairs(weights + at.col, w);
 #pragma unroll
@@ -281,11 +274,9 @@ __global__ void __launch_bounds__(MaxThreads, MaxThreads == 256 ? 2 : 1) norm_re
 #pragma unroll
             for (int c = 0; c < kPairs; ++c) {
                 r[c] = f2_fma(k[c], x[c], r[c]);
-                ss = f2_fma(r[c], r[c], ss);
                 dot = f2_fma(f2_mul(t[c], w[c]), r[c], dot);
             }
-            const float2 both = sum.two(f2_sum(ss), f2_sum(dot));
-            const float kr = exists ? root * rsqrtf(both.x + p.a.eps) : 0.f, back = kr * kr * kr * per * both.y;
+            const float back = kr * kr * kr * per * sum.one(f2_sum(dot));
 #pragma unroll
             for (int c = 0; c < kPairs; ++c) {
                 t[c] = f2_mul(t[c], f2_dup(kr));

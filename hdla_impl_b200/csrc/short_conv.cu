@@ -376,12 +376,12 @@ __global__ void __launch_bounds__(32 * kBwdWarps, WT == 8 ? 1 : 2) conv_bwd_kern
     }
 }
 
-// Strips of 32 tokens (backward also walks over W - 1 tokens behind the strip) unless too few threads would be left to keep the
-// memory busy (about 1024 an SM), then shorter ones.
+// Strips of 128 tokens unless too few threads would be left to keep the memory busy (about 1024 an SM), then shorter ones:
+// backward a strip's first and last tokens take a slower way, and it walks over W - 1 tokens behind itself.
 ConvP plan(const HdlaConvArgs& a, int warps) {
     ConvP p{};
     p.a = a;
-    p.strip = 32;
+    p.strip = 128;
     while (p.strip > 4 && (long long)a.B * ((a.T + p.strip - 1) / p.strip) * ((a.D + PW - 1) / PW) < 1024LL * sm_count()) p.strip /= 2;
     p.strips = static_cast<int>(((long long)a.T + (long long)p.strip * warps - 1) / ((long long)p.strip * warps));
     p.col_blocks = (a.D + 32 * PW - 1) / (32 * PW);

@@ -227,10 +227,12 @@ class _NormResidual(torch.autograd.Function):
         ctx.scale = None if torch.is_tensor(scale) else scale
         ctx.act, ctx.eps = act, eps
         ctx.save_for_backward(x, residual, gate, scale if ctx.scale is None else None, post_weight, pre_weight)
-        r = _lib.native().norm_residual(*_NormResidual._args(ctx, (x, residual, gate, scale, post_weight, pre_weight)))
-        if r is NotImplemented:
+        keep = any(torch.is_tensor(t) and t.requires_grad for t in (x, residual, gate, scale, post_weight, pre_weight))
+        out = _lib.native().norm_residual(*_NormResidual._args(ctx, (x, residual, gate, scale, post_weight, pre_weight)), keep)
+        if out is NotImplemented:
             raise TypeError("rms_norm_residual: unsupported arguments")
-        return r
+        r, u, ctx.factors = out
+        return r, u
 
     @staticmethod
     def _args(ctx, t):
@@ -240,7 +242,8 @@ class _NormResidual(torch.autograd.Function):
     @staticmethod
     @_op.autocast_custom_bwd
     def backward(ctx, dr, du):
-        g = _lib.native().norm_residual_backward(*_NormResidual._args(ctx, ctx.saved_tensors), _op._plain(dr), _op._plain(du))
+        g = _lib.native().norm_residual_backward(*_NormResidual._args(ctx, ctx.saved_tensors), ctx.factors,
+                                                 _op._plain(dr), _op._plain(du))
         return (*g, None, None)
 
 
@@ -265,7 +268,8 @@ def rms_norm_residual(
     if gate_act not in _GATE_ACTS:
         raise ValueError(f"gate_act {gate_act!r} must be 'sigmoid', 'silu' or None")
     act = _GATE_ACTS[gate_act]
-    out = (_lib._native or _lib.native()).norm_residual(x, residual, gate, scale, post_weight, pre_weight, act, eps)
+    out = (_lib._native or _lib.native()).norm_residual(x, residual, gate, scale, post_weight, pre_weight, act, eps,
+                                                             None)
     if out is not NotImplemented:
         return out
     vectors = {"post_weight": post_weight, "pre_weight": pre_weight, "scale": scale if torch.is_tensor(scale) else None}

@@ -359,6 +359,8 @@ typedef struct HdlaNormResidualArgs {
     int32_t reserved_;           /* keep 0                                                            */
     const void *x, *residual, *gate, *post_weight, *pre_weight, *scale;      /* all but x may be null */
     void *r, *u;                             /* forward: u null without pre_weight                    */
+    float* factors;                          /* [rows, 2]: the norms' factors, sqrt(D) / sqrt(sum a^2 + eps) after and before
+                                                the block; forward writes them (null where no backward follows), backward reads */
     const void *dr, *du;                     /* backward: either may be null (zero)                   */
     void *dx, *dresidual, *dgate;            /* null where the input is                               */
     void *dpost_weight, *dpre_weight, *dscale;       /* [D], overwritten; null where the input is      */

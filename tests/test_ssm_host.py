@@ -90,6 +90,7 @@ NO_WS = (None, C.c_size_t(1 << 30))
     ("hdla_norm_residual_fwd", norm(activation=3), (), -2, "activation"),
     ("hdla_norm_residual_fwd", norm(pre_weight=SOME), (), -1, "null"),
     ("hdla_norm_residual_bwd", norm(), WS, -3, "too small"),
+    ("hdla_norm_residual_bwd", norm(post_weight=SOME), WS, -1, "null"),
 ])
 def test_refusals_of_the_c_entry_points(name, args, more, code, text):
     rc, said = answer(name, args, *more)
