@@ -51,7 +51,7 @@ bool offsets_tensor(const Tensor& cu, int64_t B) {
     return !cu.defined() || (B == 1 && cu.dim() == 1 && cu.size(0) >= 2 && cu.size(0) <= 0x7fffffff && cu.scalar_type() == at::kLong && cu.is_contiguous());
 }
 int64_t sequences(const Tensor& cu, int64_t B) { return cu.defined() ? cu.size(0) - 1 : B; }
-// what no one can have seen yet is written by the next kernels, so a saved tensor that was changed is an error, not a result
+// A saved tensor as it was, strides included (Saved::get would make it contiguous); one that was changed since is an error.
 Tensor unpack_saved(const Saved& s, const char* node) {
     const Tensor t = s.var.unpack();
     if (!s.defined) return t;
@@ -213,8 +213,8 @@ PyObject* py_short_conv_step(PyObject*, PyObject* const* av, Py_ssize_t n) {
             HdlaConvArgs a = conv_args(i);
             y = dense({B, D}, x->scalar_type(), x->device());
             a.y = mptr(y); a.ht = mptr(*h);
+            h->unsafeGetTensorImpl()->bump_version();          // (refuses what may not be changed, before it is)
             check(ssm.conv_step(&a, stream_of(*x)), "hdla_short_conv_step");
-            h->unsafeGetTensorImpl()->bump_version();
         }))
         return nullptr;
     return wrap(y);
@@ -429,8 +429,8 @@ PyObject* py_selective_scan_step(PyObject*, PyObject* const* av, Py_ssize_t n) {
             HdlaScanArgs a = scan_args(i);
             y = dense({a.B, a.D}, c.x->scalar_type(), c.x->device());
             a.y = mptr(y); a.ht = fptr(*c.h0);
-            check(ssm.scan_step(&a, stream_of(*c.x)), "hdla_selective_scan_step");
             c.h0->unsafeGetTensorImpl()->bump_version();
+            check(ssm.scan_step(&a, stream_of(*c.x)), "hdla_selective_scan_step");
         }))
         return nullptr;
     return wrap(y);

@@ -52,7 +52,7 @@ __global__ void __launch_bounds__(kScanThreads, 5) scan_fwd_kernel(const __grid_
             nd[i] = fd.load<DT, Vec>(i, ok);
             if (has_z) nz[i] = fz.load<DT, Vec>(i, ok);
         }
-        bc.request(p.vec_bc, tokens);
+        bc.request(p.vec_bc, min(tokens, dead - t1 + tokens));   // (rows of no sequence may hold anything, and anything times 0 is not 0)
         fx.move(TB); fd.move(TB); fz.move(TB);
         bc.from.move(TB);
     };
@@ -329,13 +329,19 @@ ScanPlan scan_plan(const HdlaScanArgs& a, bool backward) {
     r.n_seg = (a.T + r.seg - 1) / r.seg;
     return r;
 }
+// Tiles of channels that keep shares of dB and dC of their own: all, unless those shares would take over 1 GiB (many states
+// make narrow tiles).  Then the tiles take turns, a launch after another, and add to the shares of those before them.
+int scan_slots(const HdlaScanArgs& a, const ScanPlan& r) {
+    const size_t each = (size_t)a.B * a.T * a.G * 8 * scan_lanes(a.N) * sizeof(float), most = (size_t(1) << 30) / each;
+    return most >= (size_t)r.tiles ? r.tiles : most < 1 ? 1 : (int)most;
+}
 ScanWork scan_work(const HdlaScanArgs& a, const ScanPlan& r, bool backward) {
     const size_t np = 4 * (size_t)scan_lanes(a.N), rows = (size_t)a.B * r.n_seg, D = a.D;
     ScanWork w{};
     auto take = [&](size_t floats) { const size_t at = w.total; w.total += up256(floats * sizeof(float)); return at; };
     if (r.n_seg > 1) { w.map_h = take(rows * D * np); w.map_d = take(rows * D); }
     if (backward) {
-        w.bc = take((size_t)r.tiles * a.B * a.T * a.G * 2 * np);
+        w.bc = take((size_t)scan_slots(a, r) * a.B * a.T * a.G * 2 * np);
         w.a = take(rows * D * np);
         w.v = take(rows * 2 * D);
     }
@@ -354,7 +360,7 @@ ScanP scan_params(const HdlaScanArgs& a, const ScanPlan& r, const ScanWork& at, 
     ScanP p{};
     p.a = a;
     p.Dg = a.D / a.G;
-    p.tiles = r.tiles; p.seg = r.seg; p.n_seg = r.n_seg;
+    p.tiles = r.tiles; p.tile_count = r.tiles; p.seg = r.seg; p.n_seg = r.n_seg;
     auto part = [&](size_t o) { return reinterpret_cast<float*>(ws + o); };
     p.map_h = part(at.map_h); p.map_d = part(at.map_d); p.part_bc = part(at.bc); p.part_a = part(at.a); p.part_v = part(at.v);
     const int bytes = a.dtype == HDLA_F32 ? 16 : 8;

@@ -24,6 +24,7 @@ constexpr int kCheckpoint = 8;                     // tokens between two saved s
 struct ScanP {
     HdlaScanArgs a;
     int Dg, tiles;             // channels of a group, tiles of channels per group
+    int first_tile, tile_count;      // those of this launch
     int seg, n_seg;            // tokens of a segment (a multiple of 16), segments
     bool vec_bc, vec_state;    // 4 states of B and C / of the states as one access
     float *map_h, *map_d;      // [B][n_seg][D][NP], [B][n_seg][D]
@@ -36,6 +37,7 @@ int scan_lanes(int N);                             // lanes that share a channel
 ScanPlan scan_plan(const HdlaScanArgs& a, bool backward);
 ScanWork scan_work(const HdlaScanArgs& a, const ScanPlan& r, bool backward);
 ScanP scan_params(const HdlaScanArgs& a, const ScanPlan& r, const ScanWork& at, unsigned char* ws);
+int scan_slots(const HdlaScanArgs& a, const ScanPlan& r);
 bool scan_vec(const HdlaScanArgs& a);              // four channels of every tensor as one access
 
 namespace {
@@ -164,9 +166,9 @@ struct Tile {
     int d0, count;                    // first channel of the tile, channels it has
     int lane, warp, nl, c0;           // this lane's first state is 4 * nl, its first channel c0 (in the tile)
     __device__ __forceinline__ explicit Tile(const ScanP& p, int segments) {
-        const int per_row = p.a.G * p.tiles;
+        const int per_row = p.a.G * p.tile_count;
         const int x = blockIdx.x % per_row, r = blockIdx.x / per_row;
-        group = x / p.tiles; tile = x % p.tiles;
+        group = x / p.tile_count; tile = p.first_tile + x % p.tile_count;
         k = r % segments; b = r / segments;
         d0 = group * p.Dg + tile * CH;
         count = min(CH, p.Dg - tile * CH);

@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(kScanThreads, Maps ? 5 : 3) scan_bwd_kernel(co
     constexpr int Parts = NL < 16 ? 16 / NL : 1, PerPass = kScanThreads / (Parts * NL);      // lanes that share an output, tokens at once
     const int out_tok = threadIdx.x / (Parts * NL), out_quad = threadIdx.x % NL, part = threadIdx.x / NL % Parts;
     const long long share_token = 2LL * p.a.G * NP;
-    float* share = Maps ? nullptr : p.part_bc + (((size_t)w.tile * p.a.B + w.b) * T + last + out_tok) * share_token + w.group * (2 * NP) +
+    float* share = Maps ? nullptr : p.part_bc + (((size_t)(w.tile - p.first_tile) * p.a.B + w.b) * T + last + out_tok) * share_token + w.group * (2 * NP) +
                                        4 * out_quad + scatter_at<4, Parts>(w.lane, NL);
     auto add_channels = [&](int tokens, int which) {
 #pragma unroll
@@ -147,7 +147,10 @@ __global__ void __launch_bounds__(kScanThreads, Maps ? 5 : 3) scan_bwd_kernel(co
             scatter_sum<4, Parts>(v, w.lane, NL);
             if (o + out_tok < tokens)
 #pragma unroll
-                for (int i = 0; i < (Parts < 4 ? 4 / Parts : 1); ++i) share[o * share_token + which * NP + i] = v[i];
+                for (int i = 0; i < (Parts < 4 ? 4 / Parts : 1); ++i) {
+                    float* to = share + o * share_token + which * NP + i;
+                    *to = p.first_tile ? *to + v[i] : v[i];
+                }
         }
     };
     const long long out0 = ((long long)w.b * T + last + tok0) * D + dch;
@@ -161,7 +164,7 @@ __global__ void __launch_bounds__(kScanThreads, Maps ? 5 : 3) scan_bwd_kernel(co
                 h[c][0] = h[c][1] = 0;
                 if (w.c0 + c < w.count) ld_quad(saved + c * NP, h[c]);
             }
-        bc.request(p.vec_bc, tokens);
+        bc.request(p.vec_bc, min(tokens, live));                 // (rows of no sequence may hold anything, and anything times 0 is not 0)
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
             const int tok = tok0 + i * Ahead, ok = tok < min(tokens, TB) ? valid : 0;
@@ -337,7 +340,7 @@ __global__ void __launch_bounds__(kScanThreads, Maps ? 5 : 3) scan_bwd_kernel(co
                     dx[c] = f2_fma(d[c], dot[c], f2_mul(skip[c], g[c]));
                     dd[c] = f2_fma(x[c], dot[c], f2_mul(dec[c], f2_dup(kLn2)));      // (A is held times log2 e)
                     if (p.a.softplus) dd[c] = f2_mul(dd[c], sigmoid_pair(f2_add(v[c], bias[c])));
-                    if (live < TB && tok >= live) dx[c] = dd[c] = dz[c] = 0;         // (g is zero)
+                    if (live < TB && tok >= live) dx[c] = dd[c] = dz[c] = x[c] = 0;  // (g is zero)
                 }
                 {
                     f2 dskip[2], dbias[2];
@@ -397,20 +400,31 @@ int selective_scan_bwd(const HdlaScanArgs& a, unsigned char* ws, cudaStream_t st
     const ScanP p = scan_params(a, r, scan_work(a, r, true), ws);
     const long long blocks = (long long)a.G * r.tiles * a.B;
     if (blocks * r.n_seg > 0x7fffffffLL) return fail(HDLA_ERR_UNSUPPORTED, "selective_scan: %lld blocks", blocks * r.n_seg);
-    for (int maps = r.n_seg > 1 ? 1 : 0; maps >= 0; --maps) {
-        const unsigned grid = static_cast<unsigned>(blocks * (r.n_seg - maps));
+    auto launch = [&](bool maps, const ScanP& part) {
+        const unsigned grid = static_cast<unsigned>((long long)a.G * part.tile_count * a.B * (r.n_seg - maps));
         with_type(a.dtype, scan_vec(a), [&](auto dt, auto vec) {
             with_lanes(scan_lanes(a.N), [&](auto nl) {
                 constexpr int ct = nl == 2 || nl == 32 ? 1 : 2;  // (as in scan_plan; two channels a lane would not fit into shared memory)
-                if (maps) scan_bwd_kernel<dt, vec, nl, ct, true><<<grid, kScanThreads, 0, st>>>(p);
-                else scan_bwd_kernel<dt, vec, nl, ct, false><<<grid, kScanThreads, 0, st>>>(p);
+                if (maps) scan_bwd_kernel<dt, vec, nl, ct, true><<<grid, kScanThreads, 0, st>>>(part);
+                else scan_bwd_kernel<dt, vec, nl, ct, false><<<grid, kScanThreads, 0, st>>>(part);
             });
         });
-        HDLA_CHECK_LAUNCH(maps ? "scan_bwd_maps_kernel" : "scan_bwd_kernel");
+    };
+    if (r.n_seg > 1) {
+        launch(true, p);
+        HDLA_CHECK_LAUNCH("scan_bwd_maps_kernel");
+    }
+    const int slots = scan_slots(a, r);
+    for (int t = 0; t < r.tiles; t += slots) {
+        ScanP part = p;
+        part.first_tile = t;
+        part.tile_count = r.tiles - t < slots ? r.tiles - t : slots;
+        launch(false, part);
+        HDLA_CHECK_LAUNCH("scan_bwd_kernel");
     }
     const int np = 4 * scan_lanes(a.N), rows = a.B * r.n_seg;
     ColJobs js{};
-    js.j[js.n++] = ColJob{p.part_bc, {a.dB, a.dC, nullptr}, (long long)a.B * a.T * a.G * 2 * np, r.tiles, 2, np, a.N, a.dtype, 0, 0, 0};
+    js.j[js.n++] = ColJob{p.part_bc, {a.dB, a.dC, nullptr}, (long long)a.B * a.T * a.G * 2 * np, slots, 2, np, a.N, a.dtype, 0, 0, 0};
     js.j[js.n++] = ColJob{p.part_a, {a.dA, nullptr, nullptr}, (long long)a.D * np, rows, 1, np, a.N, HDLA_F32, 0, 0, 0};
     if (a.dskip || a.ddt_bias)
         js.j[js.n++] = ColJob{p.part_v, {a.dskip, a.ddt_bias, nullptr}, 2LL * a.D, rows, 2, a.D, a.D, HDLA_F32, 0, 0, 0};

@@ -15,7 +15,8 @@ the steps go on with:
     y_t = selective_scan_step(x_t, dt_t, A, B_t, C_t, state, D=skip, z=z_t, dt_bias=bias)
 
 Inputs that are slices of a wider projection (dense along their last dimension) are read where they are.  Under CUDA graph
-capture give ``cu_seqlens`` as an int64 tensor on the GPU; then nothing is copied or waited for.
+capture give ``cu_seqlens`` as an int64 tensor on the GPU; then nothing is copied or waited for, and a replay goes by what the
+tensor then holds.  Rows behind the last offset may hold anything.  The gradients have no graph of their own (no double backward).
 """
 from __future__ import annotations
 
@@ -64,6 +65,7 @@ def _check_packed(x, cu) -> int:
         return x.shape[0]
     _need(x.shape[0] == 1, f"The batch size is expected to be 1 rather than {x.shape[0]} when using `cu_seqlens`.")
     _need(cu.dim() == 1 and cu.shape[0] >= 2, "cu_seqlens must be a vector of at least two offsets")
+    _lib.require_cuda(x, cu)
     return cu.shape[0] - 1
 
 

@@ -569,6 +569,88 @@ def test_offsets_that_make_no_sense_stay_inside_the_tensors(dev):
     assert torch.equal(a, b)
 
 
+def test_rows_of_no_sequence_may_hold_anything(dev):
+    """NaN and infinities behind the last offset, as memory that was never written holds them, reach nothing."""
+    from hdla_impl_b200 import ssm
+    g = gen(9)
+    for T, end in ((61, 40), (700, 330)):                          # within a tile of tokens; in segments of their own
+        cu = torch.tensor([0, 13, end], device=dev)
+        t = {k: v.to(dev) for k, v in scan_tensors(g, 1, T, 24, 16, 2, F32, "zsbph", 2).items()}
+        t["w"] = rn(g, 24, 4).to(dev)
+        dy = rn(g, 1, T, 24).to(dev)
+
+        def f(t, dy):
+            leaves = {k: v.clone().requires_grad_(True) for k, v in t.items()}
+            c, hc = ssm.short_convolution(leaves["x"], leaves["w"], output_final_state=True, cu_seqlens=cu)
+            y, hs = ssm.selective_scan(leaves["x"], leaves["dt"], leaves["A"], leaves["B"], leaves["C"], D=leaves["D"], z=leaves["z"],
+                                       dt_bias=leaves["bias"], initial_state=leaves["h0"], output_final_state=True, cu_seqlens=cu)
+            return [c, hc, y, hs, *torch.autograd.grad([c, hc, y, hs], list(leaves.values()), [dy, hc, dy, hs])]
+
+        clean = {k: v.clone() for k, v in t.items()}
+        for k in ("x", "dt", "z", "B", "C"):
+            clean[k][:, end:] = 0
+            t[k][:, end:] = float("nan")
+            t[k][:, end + 1] = float("inf")
+        cleandy = dy.clone()
+        cleandy[:, end:] = 0
+        dy[:, end:] = float("nan")
+        for a, b in zip(f(t, dy), f(clean, cleandy)):
+            assert torch.equal(a, b)
+
+
+def test_a_sequences_nan_stays_in_it(dev):
+    """A NaN in one packed sequence leaves the others' outputs, states and row gradients alone."""
+    from hdla_impl_b200 import ssm
+    g = gen(10)
+    ends = [0, 30, 75, 75, 300]
+    cu = torch.tensor(ends, device=dev)
+    t = {k: v.to(dev) for k, v in scan_tensors(g, 1, 300, 16, 5, 1, F32, "zsbph", 4).items()}
+    t["w"] = rn(g, 16, 4).to(dev)
+
+    def f(t):
+        leaves = {k: v.clone().requires_grad_(True) for k, v in t.items()}
+        c, hc = ssm.short_convolution(leaves["x"], leaves["w"], output_final_state=True, cu_seqlens=cu)
+        y, hs = ssm.selective_scan(leaves["x"], leaves["dt"], leaves["A"], leaves["B"], leaves["C"], D=leaves["D"], z=leaves["z"],
+                                   dt_bias=leaves["bias"], initial_state=leaves["h0"], output_final_state=True, cu_seqlens=cu)
+        rows = ["x", "dt", "B", "C", "z", "h0"]
+        return [c, y, hc, hs], torch.autograd.grad([c, y, hs], [leaves[k] for k in rows], [torch.ones_like(c), torch.ones_like(y), torch.ones_like(hs)])
+
+    want = f(t)
+    bad = {k: v.clone() for k, v in t.items()}
+    bad["x"][0, 40] = float("nan")
+    got = f(bad)
+    keep = torch.ones(300, dtype=torch.bool, device=dev)
+    keep[30:75] = False
+    for a, b in zip(got[0][:2] + list(got[1][:5]), want[0][:2] + list(want[1][:5])):
+        assert torch.equal(a[0, keep], b[0, keep])
+    for a, b in zip([*got[0][2:], got[1][5]], [*want[0][2:], want[1][5]]):
+        assert torch.equal(a[[0, 2, 3]], b[[0, 2, 3]])
+    assert bool(torch.isnan(got[0][3][1]).all())
+
+
+def test_shares_of_many_states_take_turns(dev):
+    """128 states and 512 channels: the tiles of four channels share the 1 GiB for their shares of dB and dC, in several launches."""
+    from hdla_impl_b200 import ssm
+    g = gen(12)
+    T, D, N = 4500, 512, 128
+    t = {k: None if v is None else v.to(dev) for k, v in scan_tensors(g, 2, T, D, N, 1, BF, "p", 2).items()}
+    dy = rn(g, 2, T, D, dtype=BF).to(dev)
+
+    def f(rows):
+        leaves = {k: (v if k == "A" else v[rows]).clone().requires_grad_(True) for k, v in t.items() if v is not None}
+        y, _ = ssm.selective_scan(leaves["x"], leaves["dt"], leaves["A"], leaves["B"], leaves["C"])
+        return torch.autograd.grad(y, list(leaves.values()), dy[rows])
+
+    whole, parts = f(slice(0, 2)), [f(slice(i, i + 1)) for i in range(2)]
+    for name, a, b, c in zip(("x", "dt", "A", "B", "C"), whole, *parts):
+        if name == "A":
+            close(a, (b.double() + c.double()).cpu(), T, name, 2 * T)
+        else:
+            # the same sums in fp32 in another order, then rounded on both sides: two half steps more
+            e = off(a, torch.cat([b, c]).cpu().double())
+            assert e <= 2 * half_step(BF) + T * 2.0 ** -21, (name, e)
+
+
 def test_checkpointing_and_subclasses(dev):
     """Recomputation gives the same bits; a tensor subclass takes the Python route and gives them too."""
     from torch.utils.checkpoint import checkpoint
