@@ -52,7 +52,7 @@ __global__ void __launch_bounds__(kScanThreads, 5) scan_fwd_kernel(const __grid_
             nd[i] = fd.load<DT, Vec>(i, ok);
             if (has_z) nz[i] = fz.load<DT, Vec>(i, ok);
         }
-        bc.request(p.vec_bc, min(tokens, dead - t1 + tokens));   // (rows of no sequence may hold anything, and anything times 0 is not 0)
+        bc.template request<Vec>(min(tokens, dead - t1 + tokens));   // (rows of no sequence may hold anything, and anything times 0 is not 0)
         fx.move(TB); fd.move(TB); fz.move(TB);
         bc.from.move(TB);
     };
@@ -218,8 +218,9 @@ __global__ void __launch_bounds__(kScanThreads, 5) scan_fwd_kernel(const __grid_
 // states' loads of Rows sequences are in flight together.  What is done once per (sequence, channel) -- softplus, gate, the
 // loads and the store of x, dt, z, y -- each lane does for one of the sequences, and hands d and d x to the others of its
 // channel: done by every lane for every sequence it was three quarters of the instructions, and took longer than the memory.
-// Bound by HBM: the fp32 state is read and written once.
-template <int DT, int NL, int Rows>
+// Bound by HBM: the fp32 state is read and written once (256 sequences of 4096 channels of 16 states: 27 us; 41 us where the
+// loads' width was a branch, see ld_state_once).
+template <int DT, int NL, int Rows, bool Vec>
 __global__ void __launch_bounds__(128) scan_step_kernel(const __grid_constant__ ScanP p) {
     static_assert(Rows == 1 || Rows <= NL, "a lane has one of the sequences");
     const int D = p.a.D, N = p.a.N, lane = threadIdx.x & 31, nl = lane % NL, n0 = 4 * nl;
@@ -232,7 +233,7 @@ __global__ void __launch_bounds__(128) scan_step_kernel(const __grid_constant__ 
     const size_t state_row = (size_t)D * N;
 #pragma unroll
     for (int r = 0; r < Rows; ++r)
-        if (r < rows) ld_state(state + r * state_row, n0, N, p.vec_state, h[r]);
+        if (r < rows) ld_state_once<Vec>(state + r * state_row, n0, N, h[r]);
     ld_state(p.a.A + (size_t)dd * N, n0, N, p.vec_state, A);
     Pack<DT, 4> rB[Rows], rC[Rows];
     const Walk fB = Walk::of<DT>(p.a.Bm, b0 * p.a.B_batch + group * p.a.B_group + n0, p.a.B_batch, 1);
@@ -240,8 +241,8 @@ __global__ void __launch_bounds__(128) scan_step_kernel(const __grid_constant__ 
 #pragma unroll
     for (int r = 0; r < Rows; ++r) {
         const int valid = r < rows ? min(4, N - n0) : 0;
-        rB[r] = p.vec_bc ? fB.load<DT, true>(r, valid) : fB.load<DT, false>(r, valid);
-        rC[r] = p.vec_bc ? fC.load<DT, true>(r, valid) : fC.load<DT, false>(r, valid);
+        rB[r] = fB.load<DT, Vec>(r, valid);
+        rC[r] = fC.load<DT, Vec>(r, valid);
     }
     // this lane's sequence of the Rows
     const int mine = scatter_at<Rows, NL>(lane, 1);
@@ -277,7 +278,7 @@ __global__ void __launch_bounds__(128) scan_step_kernel(const __grid_constant__ 
     float* to = p.a.ht + ((size_t)b0 * D + d) * N;
 #pragma unroll
     for (int r = 0; r < Rows; ++r)
-        if (r < rows) st_state(to + r * state_row, n0, N, p.vec_state, h[r]);
+        if (r < rows) st_state_once<Vec>(to + r * state_row, n0, N, h[r]);
     if (nl < Rows && mine < rows) {
         float v = fmaf(skip, x, y[0]);
         if (p.a.z) v *= z * sigmoid_of(z);
@@ -348,7 +349,10 @@ ScanWork scan_work(const HdlaScanArgs& a, const ScanPlan& r, bool backward) {
     return w;
 }
 bool scan_vec(const HdlaScanArgs& a) {
-    const int bytes = a.dtype == HDLA_F32 ? 16 : 8;              // of four channels
+    const int bytes = a.dtype == HDLA_F32 ? 16 : 8;              // of four channels or states
+    if (a.N % 4 || reinterpret_cast<uintptr_t>(a.Bm) % bytes || reinterpret_cast<uintptr_t>(a.Cm) % bytes) return false;
+    for (int64_t st : {a.B_batch, a.B_token, a.B_group, a.C_batch, a.C_token, a.C_group})
+        if (st % 4) return false;
     for (int64_t st : {a.x_batch, a.x_token, a.dt_batch, a.dt_token})
         if (st % 4) return false;
     if (a.z && (a.z_batch % 4 || a.z_token % 4)) return false;
@@ -363,9 +367,6 @@ ScanP scan_params(const HdlaScanArgs& a, const ScanPlan& r, const ScanWork& at, 
     p.tiles = r.tiles; p.tile_count = r.tiles; p.seg = r.seg; p.n_seg = r.n_seg;
     auto part = [&](size_t o) { return reinterpret_cast<float*>(ws + o); };
     p.map_h = part(at.map_h); p.map_d = part(at.map_d); p.part_bc = part(at.bc); p.part_a = part(at.a); p.part_v = part(at.v);
-    const int bytes = a.dtype == HDLA_F32 ? 16 : 8;
-    p.vec_bc = a.N % 4 == 0 && reinterpret_cast<uintptr_t>(a.Bm) % bytes == 0 && reinterpret_cast<uintptr_t>(a.Cm) % bytes == 0;
-    for (int64_t st : {a.B_batch, a.B_token, a.B_group, a.C_batch, a.C_token, a.C_group}) p.vec_bc = p.vec_bc && st % 4 == 0;
     p.vec_state = a.N % 4 == 0;
     for (const void* q : {(const void*)a.A, (const void*)a.h0, (const void*)a.ht, (const void*)a.dht, (const void*)a.dh0})
         p.vec_state = p.vec_state && aligned16(q);
@@ -408,14 +409,11 @@ int selective_scan_step(const HdlaScanArgs& a, cudaStream_t st) {
     const bool many = columns * ((a.B + rows - 1) / rows) >= 8LL * sm_count();     // several sequences a thread where enough blocks are left
     const long long grid = columns * (many ? (a.B + rows - 1) / rows : a.B);
     if (int rc = check_grid(grid)) return rc;
-    with_lanes(nl, [&](auto l) {
-        using F32 = std::integral_constant<int, HDLA_F32>;
-        using BF16 = std::integral_constant<int, HDLA_BF16>;
-        auto go = [&](auto dt) {
-            if (many) scan_step_kernel<dt, l, l == 2 ? 2 : 4><<<(unsigned)grid, 128, 0, st>>>(p);
-            else scan_step_kernel<dt, l, 1><<<(unsigned)grid, 128, 0, st>>>(p);
-        };
-        a.dtype == HDLA_F32 ? go(F32()) : go(BF16());
+    with_type(a.dtype, scan_vec(a) && p.vec_state, [&](auto dt, auto vec) {
+        with_lanes(nl, [&](auto l) {
+            if (many) scan_step_kernel<dt, l, l == 2 ? 2 : 4, vec><<<(unsigned)grid, 128, 0, st>>>(p);
+            else scan_step_kernel<dt, l, 1, vec><<<(unsigned)grid, 128, 0, st>>>(p);
+        });
     });
     HDLA_CHECK_LAUNCH("scan_step_kernel");
     return HDLA_OK;

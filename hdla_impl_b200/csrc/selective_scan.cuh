@@ -26,7 +26,7 @@ struct ScanP {
     int Dg, tiles;             // channels of a group, tiles of channels per group
     int first_tile, tile_count;      // those of this launch
     int seg, n_seg;            // tokens of a segment (a multiple of 16), segments
-    bool vec_bc, vec_state;    // 4 states of B and C / of the states as one access
+    bool vec_state;            // 4 of a channel's states as one access
     float *map_h, *map_d;      // [B][n_seg][D][NP], [B][n_seg][D]
     float *part_bc, *part_a, *part_v;      // [tiles][B][T][G][2][NP], [B * n_seg][D][NP], [B * n_seg][2][D]
 };
@@ -38,7 +38,7 @@ ScanPlan scan_plan(const HdlaScanArgs& a, bool backward);
 ScanWork scan_work(const HdlaScanArgs& a, const ScanPlan& r, bool backward);
 ScanP scan_params(const HdlaScanArgs& a, const ScanPlan& r, const ScanWork& at, unsigned char* ws);
 int scan_slots(const HdlaScanArgs& a, const ScanPlan& r);
-bool scan_vec(const HdlaScanArgs& a);              // four channels of every tensor as one access
+bool scan_vec(const HdlaScanArgs& a);              // four channels, and four states of B and C, as one access
 
 namespace {
 
@@ -149,6 +149,30 @@ __device__ __forceinline__ void st_state(float* at, int n0, int N, bool vec, con
             if (n0 + i < N) at[n0 + i] = v[i];
     }
 }
+// ... of states that pass through once (single tokens), marked as such for the caches.  Vec is known at compile time here: where
+// two ways of loading meet, the value is waited for, and the loads of several sequences would follow one another.
+template <bool Vec>
+__device__ __forceinline__ void ld_state_once(const float* at, int n0, int N, f2 (&h)[2]) {
+    if constexpr (Vec) {
+        float4 q = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (n0 < N) q = __ldcs(reinterpret_cast<const float4*>(at + n0));
+        h[0] = f2_pack(q.x, q.y);
+        h[1] = f2_pack(q.z, q.w);
+    } else {
+        ld_state(at, n0, N, false, h);
+    }
+}
+template <bool Vec>
+__device__ __forceinline__ void st_state_once(float* at, int n0, int N, const f2 (&h)[2]) {
+    if constexpr (Vec) {
+        float4 q;
+        f2_unpack(h[0], q.x, q.y);
+        f2_unpack(h[1], q.z, q.w);
+        if (n0 < N) __stcs(reinterpret_cast<float4*>(at + n0), q);
+    } else {
+        st_state(at, n0, N, false, h);
+    }
+}
 // ... of the library's own arrays, where NP states are laid out
 __device__ __forceinline__ void ld_quad(const float* at, f2 (&h)[2]) {
     const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(at);
@@ -212,11 +236,12 @@ struct BcTile {
                      : Walk::of<DT>(p.a.Bm, b * p.a.B_batch + (tb + tok) * p.a.B_token + group * p.a.B_group + 4 * quad, p.a.B_token, Ahead);
     }
     // of the tile's first `tokens` tokens (zeros behind them)
-    __device__ __forceinline__ void request(bool vec, int tokens) {
+    template <bool Vec>
+    __device__ __forceinline__ void request(int tokens) {
 #pragma unroll
         for (int i = 0; i < PerThread; ++i) {
             const int ok = tok + i * Ahead < tokens ? valid : 0;
-            raw[i] = vec ? from.load<DT, true>(i, ok) : from.load<DT, false>(i, ok);
+            raw[i] = from.load<DT, Vec>(i, ok);
         }
     }
     __device__ __forceinline__ void prefetch(int tokens) const {

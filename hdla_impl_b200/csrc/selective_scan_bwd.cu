@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(kScanThreads, Maps ? 5 : 3) scan_bwd_kernel(co
                 h[c][0] = h[c][1] = 0;
                 if (w.c0 + c < w.count) ld_quad(saved + c * NP, h[c]);
             }
-        bc.request(p.vec_bc, min(tokens, live));                 // (rows of no sequence may hold anything, and anything times 0 is not 0)
+        bc.template request<Vec>(min(tokens, live));                 // (rows of no sequence may hold anything, and anything times 0 is not 0)
 #pragma unroll
         for (int i = 0; i < IT; ++i) {
             const int tok = tok0 + i * Ahead, ok = tok < min(tokens, TB) ? valid : 0;
