@@ -10,11 +10,14 @@ namespace {
 // Maps: only the recurrence, from zero at the segment's first token (or from the initial state of a sequence that starts
 // inside it); its last state and sum of d are the segment's map.
 template <int DT, bool Vec, int NL, int CT, bool Maps>
-__global__ void __launch_bounds__(kScanThreads, 5) scan_fwd_kernel(const __grid_constant__ ScanP p) {
+__global__ void __launch_bounds__(kScanThreads, CT == 1 && !Maps ? 4 : 5) scan_fwd_kernel(const __grid_constant__ ScanP p) {
     using TileT = Tile<NL, CT>;
     constexpr int NP = TileT::NP, CH = TileT::CH, Pitch = TileT::Pitch, PW = 4;
     constexpr int TB = CH > 64 || NL >= 16 ? 8 : 16, Groups = CH / PW, Items = TB * Groups, IT = (Items + kScanThreads - 1) / kScanThreads;
     static_assert(CH % PW == 0 && kScanThreads % Groups == 0, "a thread's pieces are of one group of channels");
+    // tokens whose loads and exponentials may be mixed: sixteen with one channel a lane (eight: 616 instead of 595 us), eight with two
+    // (sixteen outgrow the registers: 922 instead of 801 us; sizes as at scan_plan)
+    constexpr int Unroll = CT == 2 ? 8 : TB;
     __shared__ __align__(16) float s_d[TB][CH], s_u[TB][CH], s_B[TB][NP], s_C[TB][NP], s_y[Maps ? 1 : TB * NL][Pitch];
 
     const int segments = Maps ? p.n_seg - 1 : p.n_seg;           // (nothing follows the last segment's map)
@@ -162,7 +165,7 @@ __global__ void __launch_bounds__(kScanThreads, 5) scan_fwd_kernel(const __grid_
         if (tokens > TB) request(tokens - TB);
         __syncthreads();
         if (end > tb + TB) {
-#pragma unroll
+#pragma unroll Unroll
             for (int j = 0; j < TB; ++j) token(j, tokens);
         } else {                                                 // a sequence ends in this tile
 #pragma unroll 1
@@ -302,10 +305,10 @@ int scan_lanes(int N) {
 // Channels a lane, and segments.  Five blocks an SM are resident forward, three backward, and about so many hide the latencies.
 // Two channels a lane are cheaper in shared-memory cycles than one, one channel a lane gives twice the blocks.  Cutting rows
 // runs the recurrence once more for the maps, and pays only where too few blocks would be left.  Measured at N = 16, 8 rows of
-// 2048 channels, T = 4096.  Forward: one channel, whole rows (512 blocks) 600 us; two channels, whole rows (256 blocks) 729 us;
+// 2048 channels, T = 4096.  Forward: one channel, whole rows (512 blocks) 573 us; two channels, whole rows (256 blocks) 729 us;
 // two channels, 16 segments 434 + 286 us for the maps.  Backward (two channels): whole rows 2070 us, 7 segments (4.04 rounds of
 // resident blocks) 1584 + 365 us, 8 segments (4.6 rounds) 1485 + 368 us, 12 segments 1489 + 365 us.  One row of 2048
-// channels, T = 65536, forward: 32 segments 1527 us, 64 segments 1443 us.  So rows are cut into segments of 64 tokens or more
+// channels, T = 65536, forward: 32 segments 1527 us, 64 segments 1389 us.  So rows are cut into segments of 64 tokens or more
 // until there are thirteen blocks an SM.
 ScanPlan scan_plan(const HdlaScanArgs& a, bool backward) {
     const int nl = scan_lanes(a.N), dg = a.D / a.G, sms = sm_count();
