@@ -5,11 +5,13 @@
 // A thread owns eight neighbouring channels of a row (16-byte accesses of bf16) and holds them, as packed pairs, between the
 // sums; a row takes as many whole warps as it needs, narrow rows share a block.  Blocks walk over rows and request the next
 // row's tensors before the sums of this one; the weights wait in shared memory, so that two (backward) or four (forward) blocks
-// of 256 threads fit on an SM: with them in registers backward had one, and took 686 instead of 300 us for 32768 rows of 2048.
+// of 256 threads fit on an SM: with them in registers backward had one, and took 686 instead of 319 us for 32768 rows of 2048.
 // Backward computes r again from the inputs in fp32 (as many bytes as reading the rounded r), reads the norms' factors that
-// forward left, takes the two sums that remain (the dot products of the norms' gradients), and keeps the sums over rows (gradients of the weights
-// and of scale) in registers until its last row; blocks' sums are added in a fixed order.  Rows of more than 4096 channels
-// need 1024 threads of 64 registers: there those sums are in shared memory too, and nothing is requested ahead.
+// forward left (305 -> 276 us: a sum and a barrier less), takes the two sums that remain (the dot products of the norms'
+// gradients), and keeps the sums over rows (gradients of the weights and of scale) in registers until its last row; blocks'
+// sums are added in a fixed order.  Rows of more than 4096 channels need 1024 threads of 64 registers: there those sums are in
+// shared memory too, and nothing is requested ahead.  32768 rows of 2048, bf16, all parts: forward 131 us = 5.1 TB/s (0.80 of
+// the measured copy), backward 271 us = 4.0 TB/s (0.61); what backward waits for is the chain of its two sums.
 #include "ssm.cuh"
 
 namespace hdla {
@@ -130,9 +132,9 @@ norm_residual_fwd_kernel(const __grid_constant__ NrP p) {
         const int ok = row < p.a.rows ? at.valid : 0;
         if (ok <= 0 && at.rows == 1) return;                // (a thread behind the row's end keeps its zeros)
         const long long i = row * D + at.col;
-        nx = ld_pack<DT, kPw, Vec>(p.a.x, i, ok);
-        if (p.a.residual) nr = ld_pack<RDT, kPw, Vec>(p.a.residual, i, ok);
-        if (p.a.gate) ng = ld_pack<DT, kPw, Vec>(p.a.gate, i, ok);
+        nx = ld_pack<DT, kPw, Vec, true>(p.a.x, i, ok);
+        if (p.a.residual) nr = ld_pack<RDT, kPw, Vec, true>(p.a.residual, i, ok);
+        if (p.a.gate) ng = ld_pack<DT, kPw, Vec, true>(p.a.gate, i, ok);
     };
     long long first = (long long)blockIdx.x * at.rows;
     const long long step = (long long)gridDim.x * at.rows;
@@ -226,11 +228,11 @@ __global__ void __launch_bounds__(MaxThreads, MaxThreads == 256 ? 2 : 1) norm_re
         const int ok = row < p.a.rows ? at.valid : 0;
         if (ok <= 0 && at.rows == 1) return;                // (a thread behind the row's end keeps its zeros)
         const long long i = row * D + at.col;
-        nx = ld_pack<DT, kPw, Vec>(p.a.x, i, ok);
-        if (p.a.residual) nr = ld_pack<RDT, kPw, Vec>(p.a.residual, i, ok);
-        if (p.a.gate) ng = ld_pack<DT, kPw, Vec>(p.a.gate, i, ok);
-        if (p.a.dr) nd = ld_pack<RDT, kPw, Vec>(p.a.dr, i, ok);
-        if (p.a.du) nu = ld_pack<DT, kPw, Vec>(p.a.du, i, ok);
+        nx = ld_pack<DT, kPw, Vec, true>(p.a.x, i, ok);
+        if (p.a.residual) nr = ld_pack<RDT, kPw, Vec, true>(p.a.residual, i, ok);
+        if (p.a.gate) ng = ld_pack<DT, kPw, Vec, true>(p.a.gate, i, ok);
+        if (p.a.dr) nd = ld_pack<RDT, kPw, Vec, true>(p.a.dr, i, ok);
+        if (p.a.du) nu = ld_pack<DT, kPw, Vec, true>(p.a.du, i, ok);
     };
     long long first = (long long)blockIdx.x * at.rows;
     const long long step = (long long)gridDim.x * at.rows;

@@ -1,7 +1,9 @@
 // Selective state space scan, forward and single tokens (the layout of the work is in selective_scan.cuh).
 //
-// What bounds the forward pass: the exponentials, one per (token, channel, state) and 16 a clock and SM, with the issue of
-// the four fused multiply-adds beside each close behind; HBM traffic takes a third of that at N = 16.
+// What bounds the forward pass: the exponentials, one per (token, channel, state) and four more per (token, channel), 16 a clock
+// and SM (62 % of their peak with two channels a lane), with shared-memory cycles (59 %) and issue slots (52 %) close behind;
+// HBM traffic takes a third of that at N = 16.  (A quarter of the exponentials as polynomials on the multiply-add pipes made
+// it slower: 835 -> 879 us.)  8 x 4096 x 2048, N = 16, bf16, with checkpoints: 575 us.
 #include "selective_scan.cuh"
 
 namespace hdla {
@@ -226,9 +228,10 @@ __global__ void __launch_bounds__(kScanThreads, CT == 1 && !Maps ? 4 : 5) scan_f
 template <int DT, int NL, int Rows, bool Vec>
 __global__ void __launch_bounds__(128) scan_step_kernel(const __grid_constant__ ScanP p) {
     static_assert(Rows == 1 || Rows <= NL, "a lane has one of the sequences");
-    const int D = p.a.D, N = p.a.N, lane = threadIdx.x & 31, nl = lane % NL, n0 = 4 * nl;
+    const int D = p.a.D, N = p.a.N, lane = threadIdx.x & 31, nl = lane % NL;
     const int blocks = (D + 128 / NL - 1) / (128 / NL);
     const int d = blockIdx.x % blocks * (128 / NL) + threadIdx.x / NL, dd = min(d, D - 1), group = dd / p.Dg;
+    const int n0 = d < D ? 4 * nl : N;                         // (lanes behind the last channel have no states)
     const long long b0 = (long long)(blockIdx.x / blocks) * Rows;
     const int rows = static_cast<int>(min((long long)Rows, p.a.B - b0));
     f2 A[2], h[Rows][2];

@@ -9,7 +9,10 @@
 // memory as partial sums, which the block's threads add; the blocks' shares of dB and dC are written per tile of channels and
 // added up in a fixed order by a last kernel, as are those of the weights.
 //
-// What bounds it: the issue of about 17 instructions per (token, channel, state), of them two exponentials (16 a clock and SM).
+// What bounds it: shared-memory cycles (62 % of their peak over the whole kernel, phases between barriers included), the issue
+// of 24 instructions per (token, channel, state) (45 %) and two exponentials (38 %), none of which overlaps the others fully
+// with the three warps a scheduler that the registers leave room for.  8 x 4096 x 2048, N = 16, bf16: 1485 us, the maps of 8
+// segments 365 us, the last kernel's sums 38 us.
 #include "selective_scan.cuh"
 
 namespace hdla {

@@ -46,16 +46,18 @@ struct Seqs {
 template <int DT, int PW>
 struct Pack { uint32_t w[PW * (DT == HDLA_F32 ? 4 : 2) / 4]; };
 
-template <int N>
+// Once: what is read for the only time is marked as such for the caches.
+template <int N, bool Once>
 __device__ __forceinline__ void ld_words(uint32_t* w, const void* p) {
     if constexpr (N % 4 == 0) {
 #pragma unroll
         for (int i = 0; i < N; i += 4) {
-            const uint4 v = *reinterpret_cast<const uint4*>(static_cast<const uint32_t*>(p) + i);
+            const uint4* at = reinterpret_cast<const uint4*>(static_cast<const uint32_t*>(p) + i);
+            const uint4 v = Once ? __ldcs(at) : *at;
             w[i] = v.x; w[i + 1] = v.y; w[i + 2] = v.z; w[i + 3] = v.w;
         }
     } else if constexpr (N == 2) {
-        const uint2 v = *static_cast<const uint2*>(p);
+        const uint2 v = Once ? __ldcs(static_cast<const uint2*>(p)) : *static_cast<const uint2*>(p);
         w[0] = v.x; w[1] = v.y;
     } else {
         w[0] = *static_cast<const uint32_t*>(p);
@@ -78,12 +80,12 @@ __device__ __forceinline__ const char* elem_ptr(const void* base, long long i) {
     return static_cast<const char*>(base) + i * (DT == HDLA_F32 ? 4 : 2);
 }
 
-template <int DT, int PW, bool Vec>
+template <int DT, int PW, bool Vec, bool Once = false>
 __device__ __forceinline__ Pack<DT, PW> ld_pack(const void* base, long long i, int valid) {
     Pack<DT, PW> r;
     constexpr int NW = sizeof(r.w) / 4;
     if constexpr (Vec) {
-        if (valid > 0) ld_words<NW>(r.w, elem_ptr<DT>(base, i));
+        if (valid > 0) ld_words<NW, Once>(r.w, elem_ptr<DT>(base, i));
         else
 #pragma unroll
             for (int j = 0; j < NW; ++j) r.w[j] = 0;

@@ -237,7 +237,8 @@ def selective_scan(
     """Selective scan over D channels of N states (1 to 128), groups of D / G channels sharing B and C:
     ``d_t = softplus(dt_t + dt_bias)``, ``h_t = exp(d_t A) h_{t-1} + d_t x_t B_t``, ``y_t = (C_t . h_t + D x_t) silu(z_t)``.
     x, dt, z, B, C are fp32 or bf16, all of one type; A, D, dt_bias and the states are used in fp32, and all arithmetic is fp32.
-    The final state is fp32.  With ``cu_seqlens`` B is 1 and n the number of sequences; rows behind the last offset give zeros."""
+    The final state is fp32.  Rows of sequences are expected to be finite (an infinite input gives NaN where the formula might
+    give an infinity).  With ``cu_seqlens`` B is 1 and n the number of sequences; rows behind the last offset give zeros."""
     cu = _offsets(cu_seqlens, x)
     softplus = bool(dt_softplus)
     r = (_lib._native or _lib.native()).selective_scan(x, dt, A, B, C, D, z, dt_bias, softplus, initial_state, cu, output_final_state, None)
