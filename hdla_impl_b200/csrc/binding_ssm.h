@@ -34,6 +34,7 @@ void bind_ssm(void* h) {
     look_up(h, "hdla_norm_residual_bwd", ssm.norm_bwd);
 }
 
+const float* read(const Tensor& t) { return static_cast<const float*>(ptr(t)); }
 cudaStream_t stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
 // Rows may lie anywhere as long as a row's last dimension is dense: slices of a wider projection are read where they are.
 Tensor rows_of(const Tensor& t) { return !t.defined() || t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
@@ -209,8 +210,12 @@ PyObject* py_short_conv_step(PyObject*, PyObject* const* av, Py_ssize_t n) {
     if (!guarded([&] {
             at::NoGradGuard no_grad;
             c10::cuda::CUDAGuard guard(x->device());
-            const ConvIn i{rows_of(*x).unsqueeze(1), w->contiguous(), b->defined() ? as_type(*b, w->scalar_type()).contiguous() : *b, *h, Tensor(), silu != 0};
-            HdlaConvArgs a = conv_args(i);
+            const Tensor xr = rows_of(*x), wc = w->contiguous(), bc = b->defined() ? as_type(*b, w->scalar_type()).contiguous() : *b;
+            HdlaConvArgs a{};                                  // (filled in here: views of one token cost more than the call)
+            a.B = (int)B; a.T = 1; a.D = (int)D; a.W = (int)W;
+            a.dtype = dtype_code(xr); a.w_dtype = dtype_code(wc); a.activation = silu ? HDLA_ACT_SILU : HDLA_ACT_NONE;
+            a.x_batch = step_of(xr, 0);
+            a.x = ptr(xr); a.weight = ptr(wc); a.bias = ptr(bc); a.h0 = ptr(*h);
             y = dense({B, D}, x->scalar_type(), x->device());
             a.y = mptr(y); a.ht = mptr(*h);
             h->unsafeGetTensorImpl()->bump_version();          // (refuses what may not be changed, before it is)
@@ -235,7 +240,7 @@ HdlaScanArgs scan_args(const ScanIn& i) {
     a.B_batch = step_of(i.B, 0); a.B_token = step_of(i.B, 1); a.B_group = step_of(i.B, 2);
     a.C_batch = step_of(i.C, 0); a.C_token = step_of(i.C, 1); a.C_group = step_of(i.C, 2);
     a.x = ptr(i.x); a.dt = ptr(i.dt); a.z = ptr(i.z); a.Bm = ptr(i.B); a.Cm = ptr(i.C);
-    a.A = fptr(i.A); a.skip = fptr(i.D); a.dt_bias = fptr(i.bias); a.h0 = fptr(i.h0);
+    a.A = read(i.A); a.skip = read(i.D); a.dt_bias = read(i.bias); a.h0 = read(i.h0);
     return a;
 }
 // B and C as [B, T, G, N]
@@ -265,7 +270,7 @@ ScanGrads scan_backward(const ScanIn& i, const Tensor& ckpt, const Tensor& dy_, 
     const size_t n = ssm.scan_bytes(&a, 1);
     const Tensor ws = space(n, i.x);
     a.checkpoints = fptr(ckpt);
-    a.dy = ptr(dy); a.dht = fptr(dht);
+    a.dy = ptr(dy); a.dht = read(dht);
     a.dx = mptr(g.dx); a.ddt = mptr(g.ddt); a.dz = mptr(g.dz); a.dB = mptr(g.dB); a.dC = mptr(g.dC);
     a.dA = fptr(g.dA); a.dskip = fptr(g.dD); a.ddt_bias = fptr(g.dbias); a.dh0 = fptr(g.dh0);
     check(ssm.scan_bwd(&a, mptr(ws), n, stream_of(i.x)), "hdla_selective_scan_bwd");
@@ -422,11 +427,16 @@ PyObject* py_selective_scan_step(PyObject*, PyObject* const* av, Py_ssize_t n) {
     if (!guarded([&] {
             at::NoGradGuard no_grad;
             c10::cuda::CUDAGuard guard(c.x->device());
-            auto token = [](const Tensor& t) { return t.defined() ? rows_of(t).unsqueeze(1) : t; };
-            auto bc = [](const Tensor& t) { return rows_of(t.dim() == 2 ? t.unsqueeze(1) : t).unsqueeze(1); };
-            const ScanIn i{token(*c.x), token(*c.dt), f32_contiguous(*c.A), bc(*c.B), bc(*c.C), f32_contiguous(*c.D), token(*c.z),
-                           f32_contiguous(*c.bias), *c.h0, Tensor(), c.softplus};
-            HdlaScanArgs a = scan_args(i);
+            const Tensor x = rows_of(*c.x), dt = rows_of(*c.dt), z = rows_of(*c.z), B = rows_of(*c.B), C = rows_of(*c.C),
+                         A = f32_contiguous(*c.A), D = f32_contiguous(*c.D), bias = f32_contiguous(*c.bias);
+            HdlaScanArgs a{};                                  // (filled in here: views of one token cost more than the call)
+            a.B = (int)x.size(0); a.T = 1; a.D = (int)x.size(1); a.N = (int)A.size(1); a.G = B.dim() == 3 ? (int)B.size(1) : 1;
+            a.dtype = dtype_code(x); a.softplus = c.softplus;
+            a.x_batch = step_of(x, 0); a.dt_batch = step_of(dt, 0); a.z_batch = z.defined() ? step_of(z, 0) : 0;
+            a.B_batch = step_of(B, 0); a.C_batch = step_of(C, 0);
+            if (B.dim() == 3) { a.B_group = step_of(B, 1); a.C_group = step_of(C, 1); }
+            a.x = ptr(x); a.dt = ptr(dt); a.z = ptr(z); a.Bm = ptr(B); a.Cm = ptr(C);
+            a.A = read(A); a.skip = read(D); a.dt_bias = read(bias); a.h0 = read(*c.h0);
             y = dense({a.B, a.D}, c.x->scalar_type(), c.x->device());
             a.y = mptr(y); a.ht = fptr(*c.h0);
             c.h0->unsafeGetTensorImpl()->bump_version();

@@ -250,7 +250,6 @@ class _NormResidual(torch.autograd.Function):
 _GATE_ACTS = {None: 0, "silu": 1, "sigmoid": 2}
 
 
-@torch.compiler.disable
 def rms_norm_residual(
     x: torch.Tensor,                                # [..., D]  a block's output
     residual: Optional[torch.Tensor] = None,        # [..., D]  of x's type, or fp32

@@ -173,7 +173,6 @@ def _silu(activation) -> bool:
     return _ACTIVATIONS[activation]
 
 
-@torch.compiler.disable
 def short_convolution(
     x: torch.Tensor,                               # [B, T, D]
     weight: torch.Tensor,                          # [D, W]
@@ -196,7 +195,6 @@ def short_convolution(
     return _ShortConv.apply(x, weight, bias, silu, initial_state, cu, bool(output_final_state))
 
 
-@torch.compiler.disable
 def short_convolution_step(
     x: torch.Tensor,                               # [B, D]
     state: torch.Tensor,                           # [B, W-1, D], updated in place
@@ -219,7 +217,6 @@ def short_convolution_step(
     return r
 
 
-@torch.compiler.disable
 def selective_scan(
     x: torch.Tensor,                               # [B, T, D]
     dt: torch.Tensor,                              # [B, T, D]
@@ -249,7 +246,6 @@ def selective_scan(
     return _SelectiveScan.apply(x, dt, A, B, C, D, z, dt_bias, softplus, initial_state, cu, bool(output_final_state))
 
 
-@torch.compiler.disable
 def selective_scan_step(
     x: torch.Tensor,                               # [B, D]
     dt: torch.Tensor,                              # [B, D]
