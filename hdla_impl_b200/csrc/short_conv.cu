@@ -6,7 +6,7 @@
 // has just brought to L2.  Several tokens are requested at a time, and forward the next ones before these are worked on.  Four
 // channels a thread and not eight (16 bytes of bf16): the taps, their sums and the histories are what fills the registers, and
 // with half of them twice the warps hide the latency (forward 100 -> 61 us, backward 262 -> 148 us at 32768 x 2048, W = 4).
-// There forward now takes 60 us = 4.5 TB/s (0.69 of the measured copy), backward 104 us = 3.9 TB/s and its sums 10 us.
+// There forward now takes 55 us = 4.9 TB/s (0.76 of the measured copy), backward 104 us = 3.9 TB/s (0.60) and its sums 10 us.
 #include "ssm.cuh"
 
 namespace hdla {
@@ -120,7 +120,7 @@ __device__ __forceinline__ void store_state(const ConvP& p, long long state, int
 
 template <int DT, int WT, bool Vec>
 __global__ void __launch_bounds__(32 * kFwdWarps) conv_fwd_kernel(const __grid_constant__ ConvP p) {
-    constexpr int U = 4;
+    constexpr int U = 8;                                       // tokens requested ahead (four: 60 us instead of 55 at 32768 x 2048)
     const int T = p.a.T, D = p.a.D, W = WT == 8 ? p.a.W : WT;
     const int cb = blockIdx.x % p.col_blocks, sb = blockIdx.x / p.col_blocks % p.strips, b = blockIdx.x / p.col_blocks / p.strips;
     const int ch = (cb * 32 + (threadIdx.x & 31)) * PW, valid = min(PW, D - ch);
