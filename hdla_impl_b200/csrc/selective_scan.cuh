@@ -6,9 +6,10 @@
 // Layout of the work.  A warp holds the states of (32 / NL) * CT channels in registers: NL lanes share a channel's states,
 // four a lane, and a lane has CT channels, so that one 16-byte read of B (and C) serves 4 * CT states.  Four warps make a
 // block; it walks over its tokens in tiles, in three steps: what is done once per (token, channel) -- softplus, d x, gates --
-// by all threads on pieces of four channels into shared memory; the recurrence; the outputs.  Sums over n are left in shared memory as NL partial sums, which the threads of
-// the third step add: fewer instructions than shuffles and selects.  The next tile's inputs are requested before the
-// recurrence of this one.  All arithmetic is fp32, the outputs are rounded once.
+// by all threads on pieces of four channels into shared memory; the recurrence; the outputs.  Sums over n are left in shared
+// memory as NL partial sums, which the threads of the third step add: fewer instructions than shuffles and selects.  The next
+// tile's inputs are requested before the recurrence of this one (backward: brought to L2).  All arithmetic is fp32, the
+// outputs are rounded once.
 //
 // Long rows of few channels are cut into segments.  What a segment does to a state is exp(A sum d) h + F, and its sum of d
 // and F come from a first kernel that runs the recurrence alone, from zero; the second kernel's blocks chain the maps of

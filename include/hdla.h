@@ -277,8 +277,8 @@ HDLA_API int hdla_norm_gate_bwd(const void* x, const void* gate, const void* wei
  *
  * Every call takes one argument struct.  Activations share `dtype` (HDLA_F32 or HDLA_BF16); channels lie next to each
  * other, the strides between sequences (`*_batch`) and tokens (`*_token`) are given in elements where an input may be a
- * slice of a wider tensor, and outputs, gradients and states are dense.  Any size and any element alignment is taken;
- * 16-byte aligned tensors whose strides are multiples of 16 bytes run faster.
+ * slice of a wider tensor, and outputs, gradients and states are dense.  Any size and any element alignment is taken; tensors
+ * that start at a multiple of 16 bytes, with channels, states and strides in multiples of four (norms: eight), run faster.
  *
  * Packed batches: with cu_seqlens (DEVICE array of n_seqs + 1 offsets that do not decrease; its first entry counts as
  * 0) B is 1, sequence s holds tokens [cu_seqlens[s], cu_seqlens[s+1]) and has state s.  Sequences may be empty: their

@@ -531,6 +531,38 @@ def test_a_training_pass_is_captured_and_replayed_on_new_inputs(dev):
         assert torch.equal(a, b)
 
 
+def test_single_tokens_are_captured_and_replayed(dev):
+    """A decode step in a graph moves the states on at every replay, as the calls themselves do."""
+    from hdla_impl_b200 import layer_ops, ssm
+    g = gen(13)
+    B, D, N = 5, 72, 16
+    t = {k: v.to(dev) for k, v in scan_tensors(g, B, 1, D, N, 1, BF, "zsbp", B).items() if v is not None}
+    w = rn(g, D, 4, dtype=BF).to(dev)
+    x, dt, z, Bm, Cm = (t[k][:, 0].clone() for k in ("x", "dt", "z", "B", "C"))
+    states = [[torch.zeros(B, 3, D, dtype=BF, device=dev), torch.zeros(B, D, N, device=dev)] for _ in range(2)]
+
+    def f(conv, scan):
+        c = ssm.short_convolution_step(x, conv, w)
+        y = ssm.selective_scan_step(c, dt, t["A"], Bm, Cm, scan, D=t["D"], z=z, dt_bias=t["bias"])
+        return layer_ops.rms_norm_residual(y, x, pre_weight=w[:, 0])[1]
+
+    side = torch.cuda.Stream(dev)
+    with torch.no_grad(), torch.cuda.stream(side):
+        f(*[s.clone() for s in states[0]])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.no_grad(), torch.cuda.graph(graph, stream=side):
+        out = f(*states[0])
+    for i in range(4):
+        x.copy_(rn(g, B, D, dtype=BF))
+        graph.replay()
+        torch.cuda.synchronize()
+        with torch.no_grad():
+            assert torch.equal(f(*states[1]), out)
+    for a, b in zip(*states):
+        assert torch.equal(a, b)
+
+
 def test_an_eager_graph_that_lives_on_does_not_disturb_a_captured_backward(dev):
     """The leaves' eager graph (made on the capturing stream, as a training loop makes it) is kept while a backward pass of the same
     leaves is captured, and used after that."""
