@@ -15,6 +15,7 @@ namespace {
 constexpr int PW = 4;
 constexpr int kFwdWarps = 4, kBwdWarps = 8;
 struct Quad { f2 v[2]; };                                        // four channels
+template <int WT> constexpr int kHist = WT > 1 ? WT - 1 : 1;     // rows of history (one, of no use, with a single tap)
 
 struct ConvP {
     HdlaConvArgs a;
@@ -40,10 +41,9 @@ __device__ __forceinline__ void st_quad(void* base, long long i, int valid, cons
 // w[k]: the weights of lag k for the thread's channels
 template <int WT, bool Vec>
 __device__ __forceinline__ void load_taps(const ConvP& p, int ch, int valid, Quad (&w)[WT], Quad& bias) {
-    const int W = WT == 8 ? p.a.W : WT;
     float f[PW][WT], b[PW];
     bool done = false;
-    if constexpr (Vec && WT != 8 && PW * WT % 8 == 0) {
+    if constexpr (Vec && PW * WT % 8 == 0) {
         if (p.wide_w) {
             if (p.a.w_dtype == HDLA_BF16)
                 unpack<HDLA_BF16, PW * WT>(ld_pack<HDLA_BF16, PW * WT, true>(p.a.weight, (long long)ch * WT, 1), &f[0][0]);
@@ -56,34 +56,25 @@ __device__ __forceinline__ void load_taps(const ConvP& p, int ch, int valid, Qua
     for (int c = 0; c < PW; ++c) {
         if (!done)
 #pragma unroll
-            for (int j = 0; j < WT; ++j) f[c][j] = c < valid && j < W ? ld_elem(p.a.weight, (size_t)(ch + c) * W + j, p.a.w_dtype) : 0.f;
+            for (int j = 0; j < WT; ++j) f[c][j] = c < valid ? ld_elem(p.a.weight, (size_t)(ch + c) * WT + j, p.a.w_dtype) : 0.f;
         b[c] = p.a.bias && c < valid ? ld_elem(p.a.bias, ch + c, p.a.w_dtype) : 0.f;
     }
 #pragma unroll
     for (int k = 0; k < WT; ++k) {
-        float t[PW];
-#pragma unroll
-        for (int c = 0; c < PW; ++c) {
-            t[c] = 0.f;
-#pragma unroll
-            for (int j = 0; j < WT; ++j)
-                if (WT != 8 ? j == WT - 1 - k : j == W - 1 - k) t[c] = f[c][j];
-        }
-        w[k] = Quad{{f2_pack(t[0], t[1]), f2_pack(t[2], t[3])}};
+        const int j = WT - 1 - k;
+        w[k] = Quad{{f2_pack(f[0][j], f[1][j]), f2_pack(f[2][j], f[3][j])}};
     }
     bias = Quad{{f2_pack(b[0], b[1]), f2_pack(b[2], b[3])}};
 }
 
-// Taps beyond W (only with WT == 8) are left out, not multiplied by zero: what they would read may be infinite.
 template <int WT>
-__device__ __forceinline__ Quad taps(const Quad (&w)[WT], const Quad& bias, const Quad& x, const Quad (&hist)[WT - 1], int W) {
+__device__ __forceinline__ Quad taps(const Quad (&w)[WT], const Quad& bias, const Quad& x, const Quad (&hist)[kHist<WT>]) {
     Quad out;
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
         f2 s = f2_fma(w[0].v[c], x.v[c], bias.v[c]);
 #pragma unroll
-        for (int k = 1; k < WT; ++k)
-            if (WT != 8 || k < W) s = f2_fma(w[k].v[c], hist[k - 1].v[c], s);
+        for (int k = 1; k < WT; ++k) s = f2_fma(w[k].v[c], hist[k - 1].v[c], s);
         out.v[c] = s;
     }
     return out;
@@ -97,31 +88,29 @@ __device__ __forceinline__ void shift(Quad (&hist)[N], const Quad& x) {
 
 // The inputs of the W - 1 tokens before token t of a sequence that starts at `start`: its initial state's rows before that.
 template <int DT, int WT, bool Vec>
-__device__ __forceinline__ void load_hist(const ConvP& p, long long xrow, long long state, int start, int t, int ch, int valid, Quad (&hist)[WT - 1]) {
-    const int W = WT == 8 ? p.a.W : WT;
+__device__ __forceinline__ void load_hist(const ConvP& p, long long xrow, long long state, int start, int t, int ch, int valid, Quad (&hist)[kHist<WT>]) {
+    constexpr int W = WT;
+    hist[0] = Quad{{0, 0}};
 #pragma unroll
     for (int k = 0; k < WT - 1; ++k) {
         const int tt = t - 1 - k;
         Pack<DT, PW> r = {};
-        if (k < W - 1) {
-            if (tt >= start) r = ld_pack<DT, PW, Vec>(p.a.x, xrow + tt * p.a.x_token + ch, valid);
-            else if (p.a.h0) r = ld_pack<DT, PW, Vec>(p.a.h0, (state * (W - 1) + (W - 1 + tt - start)) * p.a.D + ch, valid);
-        }
+        if (tt >= start) r = ld_pack<DT, PW, Vec>(p.a.x, xrow + tt * p.a.x_token + ch, valid);
+        else if (p.a.h0) r = ld_pack<DT, PW, Vec>(p.a.h0, (state * (W - 1) + (W - 1 + tt - start)) * p.a.D + ch, valid);
         hist[k] = quad_of<DT>(r);
     }
 }
 template <int DT, int WT, bool Vec>
-__device__ __forceinline__ void store_state(const ConvP& p, long long state, int ch, int valid, const Quad (&hist)[WT - 1]) {
-    const int W = WT == 8 ? p.a.W : WT;
+__device__ __forceinline__ void store_state(const ConvP& p, long long state, int ch, int valid, const Quad (&hist)[kHist<WT>]) {
+    constexpr int W = WT;
 #pragma unroll
-    for (int k = 0; k < WT - 1; ++k)
-        if (k < W - 1) st_quad<DT, Vec>(p.a.ht, (state * (W - 1) + (W - 2 - k)) * p.a.D + ch, valid, hist[k]);
+    for (int k = 0; k < WT - 1; ++k) st_quad<DT, Vec>(p.a.ht, (state * (W - 1) + (W - 2 - k)) * p.a.D + ch, valid, hist[k]);
 }
 
 template <int DT, int WT, bool Vec>
 __global__ void __launch_bounds__(32 * kFwdWarps) conv_fwd_kernel(const __grid_constant__ ConvP p) {
     constexpr int U = 8;                                       // tokens requested ahead (four: 60 us instead of 55 at 32768 x 2048)
-    const int T = p.a.T, D = p.a.D, W = WT == 8 ? p.a.W : WT;
+    const int T = p.a.T, D = p.a.D;
     const int cb = blockIdx.x % p.col_blocks, sb = blockIdx.x / p.col_blocks % p.strips, b = blockIdx.x / p.col_blocks / p.strips;
     const int ch = (cb * 32 + (threadIdx.x & 31)) * PW, valid = min(PW, D - ch);
     const long long first = ((long long)sb * kFwdWarps + (threadIdx.x >> 5)) * p.strip;
@@ -140,7 +129,7 @@ __global__ void __launch_bounds__(32 * kFwdWarps) conv_fwd_kernel(const __grid_c
         from += U * from_step;
     };
     request(t1 - t0);
-    Quad w[WT], bias, hist[WT - 1];
+    Quad w[WT], bias, hist[kHist<WT>];
     load_taps<WT, Vec>(p, ch, valid, w, bias);
     int s = q.ends_behind(t0);
     if (t0 == 0 && p.a.ht)
@@ -156,7 +145,7 @@ __global__ void __launch_bounds__(32 * kFwdWarps) conv_fwd_kernel(const __grid_c
         if (t + U < t1) request(t1 - t - U);
         auto one = [&](int u) {
             const Quad x = quad_of<DT>(in[u]);
-            Quad out = taps<WT>(w, bias, x, hist, W);
+            Quad out = taps<WT>(w, bias, x, hist);
             if (p.a.activation == HDLA_ACT_SILU)
 #pragma unroll
                 for (int c = 0; c < 2; ++c) out.v[c] = f2_mul(out.v[c], sigmoid_pair(out.v[c]));
@@ -191,17 +180,17 @@ __global__ void __launch_bounds__(32 * kFwdWarps) conv_fwd_kernel(const __grid_c
 // One token: the state is the history, and moves on by one row in place (a thread owns its channels' rows).
 template <int DT, int WT, bool Vec>
 __global__ void __launch_bounds__(128) conv_step_kernel(const __grid_constant__ ConvP p) {
-    const int D = p.a.D, W = WT == 8 ? p.a.W : WT;
+    const int D = p.a.D;
     const int cb = blockIdx.x % p.col_blocks;
     const long long b = (long long)(blockIdx.x / p.col_blocks) * 4 + (threadIdx.x >> 5);
     const int ch = (cb * 32 + (threadIdx.x & 31)) * PW, valid = min(PW, D - ch);
     if (valid <= 0 || b >= p.a.B) return;
-    Quad w[WT], bias, hist[WT - 1];
+    Quad w[WT], bias, hist[kHist<WT>];
     const Pack<DT, PW> in = ld_pack<DT, PW, Vec>(p.a.x, b * p.a.x_batch + ch, valid);
     load_hist<DT, WT, Vec>(p, 0, b, 0, 0, ch, valid, hist);
     load_taps<WT, Vec>(p, ch, valid, w, bias);
     const Quad x = quad_of<DT>(in);
-    Quad out = taps<WT>(w, bias, x, hist, W);
+    Quad out = taps<WT>(w, bias, x, hist);
     if (p.a.activation == HDLA_ACT_SILU)
 #pragma unroll
         for (int c = 0; c < 2; ++c) out.v[c] = f2_mul(out.v[c], sigmoid_pair(out.v[c]));
@@ -214,11 +203,13 @@ __global__ void __launch_bounds__(128) conv_step_kernel(const __grid_constant__ 
 // Walking forward, the row that a token completes is the one W - 1 before it, so the gradient of the initial state comes out
 // as the rows before a sequence's start, and the final state's gradient joins the last W - 1 rows, which W - 1 more steps
 // with dp = 0 complete.  A strip also walks over the W - 1 tokens behind it, for its own last rows.
+// Two blocks an SM where the registers of that many taps allow it (16384 x 2048, W = 4, bf16: 64 us, with one block 80 us; fp32
+// spills with two, 165 us, with one 100 us).
 template <int DT, int WT, bool Vec>
-__global__ void __launch_bounds__(32 * kBwdWarps, WT == 8 ? 1 : 2) conv_bwd_kernel(const __grid_constant__ ConvP p) {
-    constexpr int U = 4;
+__global__ void __launch_bounds__(32 * kBwdWarps, WT <= (DT == HDLA_F32 ? 2 : 4) ? 2 : 1) conv_bwd_kernel(const __grid_constant__ ConvP p) {
+    constexpr int U = 4, W = WT;
     __shared__ __align__(16) float red[kBwdWarps][WT + 1][32 * PW];
-    const int T = p.a.T, D = p.a.D, W = WT == 8 ? p.a.W : WT;
+    const int T = p.a.T, D = p.a.D;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int cb = blockIdx.x % p.col_blocks, sb = blockIdx.x / p.col_blocks % p.strips, b = blockIdx.x / p.col_blocks / p.strips;
     const int ch = (cb * 32 + lane) * PW, valid = min(PW, D - ch);
@@ -232,7 +223,7 @@ __global__ void __launch_bounds__(32 * kBwdWarps, WT == 8 ? 1 : 2) conv_bwd_kern
 #pragma unroll
     for (int k = 0; k < WT; ++k) dw[k] = Quad{{0, 0}};
     if (valid > 0 && first < T) {
-        Quad w[WT], bias, xh[WT - 1], dph[WT - 1];
+        Quad w[WT], bias, xh[kHist<WT>], dph[kHist<WT>];
         load_taps<WT, Vec>(p, ch, valid, w, bias);
         const int t0 = static_cast<int>(first), t1 = min(T, t0 + p.strip);
         int s = q.ends_behind(t0), start = 0, end = 0, from = 0;
@@ -243,16 +234,7 @@ __global__ void __launch_bounds__(32 * kBwdWarps, WT == 8 ? 1 : 2) conv_bwd_kern
             for (int c = 0; c < 2; ++c) {
                 f2 r = 0;
 #pragma unroll
-                for (int k = 0; k < WT; ++k) {
-                    if (WT != 8) r = f2_fma(w[k].v[c], k == WT - 1 ? dp.v[c] : dph[WT - 2 - k < 0 ? 0 : WT - 2 - k].v[c], r);
-                    else if (k < W) {
-                        f2 d = dp.v[c];
-#pragma unroll
-                        for (int i = 0; i < WT - 1; ++i)
-                            if (i == W - 2 - k) d = dph[i].v[c];
-                        r = f2_fma(w[k].v[c], d, r);
-                    }
-                }
+                for (int k = 0; k < WT; ++k) r = f2_fma(w[k].v[c], k == WT - 1 ? dp.v[c] : dph[WT - 2 - k < 0 ? 0 : WT - 2 - k].v[c], r);
                 v.v[c] = r;
             }
             shift(dph, dp);
@@ -277,7 +259,7 @@ __global__ void __launch_bounds__(32 * kBwdWarps, WT == 8 ? 1 : 2) conv_bwd_kern
             const Quad x = quad_of<DT>(xin);
             Quad dp = quad_of<DT>(yin);
             if (silu) {
-                const Quad pre = taps<WT>(w, bias, x, xh, W);
+                const Quad pre = taps<WT>(w, bias, x, xh);
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {                  // silu' = s + p s (1 - s)
                     const f2 sg = sigmoid_pair(pre.v[c]), ps = f2_mul(pre.v[c], sg);
@@ -290,15 +272,14 @@ __global__ void __launch_bounds__(32 * kBwdWarps, WT == 8 ? 1 : 2) conv_bwd_kern
                     db.v[c] = f2_add(db.v[c], dp.v[c]);
                     dw[0].v[c] = f2_fma(dp.v[c], x.v[c], dw[0].v[c]);
 #pragma unroll
-                    for (int k = 1; k < WT; ++k)
-                        if (WT != 8 || k < W) dw[k].v[c] = f2_fma(dp.v[c], xh[k - 1].v[c], dw[k].v[c]);
+                    for (int k = 1; k < WT; ++k) dw[k].v[c] = f2_fma(dp.v[c], xh[k - 1].v[c], dw[k].v[c]);
                 }
             shift(xh, x);
             return dp;
         };
         auto clear = [&] {
 #pragma unroll
-            for (int k = 0; k < WT - 1; ++k) dph[k] = Quad{{0, 0}};
+            for (int k = 0; k < kHist<WT>; ++k) dph[k] = Quad{{0, 0}};
         };
         const Quad none = {{0, 0}};
         auto empty = [&](int i, int at) {                      // an empty sequence at token `at`: dh0 = dht
@@ -398,10 +379,16 @@ bool conv_vec(const HdlaConvArgs& a) {
 
 template <typename F>
 void with_taps(int W, F f) {
-    if (W == 2) f(std::integral_constant<int, 2>());
-    else if (W == 3) f(std::integral_constant<int, 3>());
-    else if (W == 4) f(std::integral_constant<int, 4>());
-    else f(std::integral_constant<int, 8>());
+    switch (W) {
+        case 1: return f(std::integral_constant<int, 1>());
+        case 2: return f(std::integral_constant<int, 2>());
+        case 3: return f(std::integral_constant<int, 3>());
+        case 4: return f(std::integral_constant<int, 4>());
+        case 5: return f(std::integral_constant<int, 5>());
+        case 6: return f(std::integral_constant<int, 6>());
+        case 7: return f(std::integral_constant<int, 7>());
+        default: return f(std::integral_constant<int, 8>());
+    }
 }
 template <typename F>
 void with_type(int dtype, bool vec, F f) {
