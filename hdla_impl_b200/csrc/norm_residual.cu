@@ -51,14 +51,71 @@ struct RowSum {
     }
 };
 
-// Where a thread stands.
+// Where a thread stands.  Its eight channels are neighbours where a row can be read in 16-byte pieces (Vec); else they lie
+// per_row apart, so that neighbouring threads read neighbouring channels (4096 bf16 rows of 8191 channels, backward: 378 us;
+// with neighbours for each thread there too 556 us).
+template <bool Vec>
 struct Place {
-    int rows, group, col, valid;
-    __device__ __forceinline__ explicit Place(const NrP& p) {
-        rows = blockDim.x / p.per_row;
-        group = threadIdx.x / p.per_row;
-        col = (threadIdx.x % p.per_row) * kPw;
-        valid = max(0, min(kPw, p.a.D - col));
+    int rows, group, lane, per_row, D;
+    int col, valid;                                             // (Vec)
+    __device__ __forceinline__ explicit Place(const NrP& p) : per_row(p.per_row), D(p.a.D) {
+        rows = blockDim.x / per_row;
+        group = threadIdx.x / per_row;
+        lane = threadIdx.x % per_row;
+        col = lane * kPw;
+        valid = max(0, min(kPw, D - col));
+    }
+    __device__ __forceinline__ bool any() const { return Vec ? valid > 0 : lane < D; }
+    template <int DT>
+    __device__ __forceinline__ Pack<DT, kPw> load(const void* base, long long row, bool exists) const {
+        if constexpr (Vec) {
+            return ld_pack<DT, kPw, true, true>(base, row * D + col, exists ? valid : 0);
+        } else {
+            Pack<DT, kPw> r = {};
+#pragma unroll
+            for (int c = 0; c < kPw; ++c) {
+                const int col = lane + c * per_row;
+                if (!exists || col >= D) continue;
+                if constexpr (DT == HDLA_F32) r.w[c] = static_cast<const uint32_t*>(base)[row * D + col];
+                else r.w[c / 2] |= static_cast<uint32_t>(static_cast<const uint16_t*>(base)[row * D + col]) << (c % 2 * 16);
+            }
+            return r;
+        }
+    }
+    template <int DT>
+    __device__ __forceinline__ void store(void* base, long long row, bool exists, const f2 (&v)[kPairs]) const {
+        float f[kPw];
+#pragma unroll
+        for (int c = 0; c < kPairs; ++c) f2_unpack(v[c], f[2 * c], f[2 * c + 1]);
+        if constexpr (Vec) {
+            st_pack<DT, kPw, true>(base, row * D + col, exists ? valid : 0, f);
+        } else {
+#pragma unroll
+            for (int c = 0; c < kPw; ++c)
+                if (exists && lane + c * per_row < D) st_elem(base, row * D + lane + c * per_row, DT, f[c]);
+        }
+    }
+    // this thread's channels of a vector in shared memory
+    __device__ __forceinline__ void get(const float* vector, f2 (&v)[kPairs]) const {
+        if constexpr (Vec) {
+#pragma unroll
+            for (int i = 0; i < kPairs; i += 2) {
+                const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(vector + col + 2 * i);
+                v[i] = q.x; v[i + 1] = q.y;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kPairs; ++i) v[i] = f2_pack(vector[lane + 2 * i * per_row], vector[lane + (2 * i + 1) * per_row]);
+        }
+    }
+    __device__ __forceinline__ void put(float* vector, const f2 (&v)[kPairs]) const {
+        if constexpr (Vec) {
+#pragma unroll
+            for (int i = 0; i < kPairs; i += 2) *reinterpret_cast<ulonglong2*>(vector + col + 2 * i) = make_ulonglong2(v[i], v[i + 1]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kPairs; ++i) f2_unpack(v[i], vector[lane + 2 * i * per_row], vector[lane + (2 * i + 1) * per_row]);
+        }
     }
 };
 
@@ -72,17 +129,6 @@ __device__ __forceinline__ void put_weights(const NrP& p, float* to) {
     }
     __syncthreads();
 }
-__device__ __forceinline__ void ld_pairs(const float* at, f2 (&v)[kPairs]) {
-#pragma unroll
-    for (int i = 0; i < kPairs; i += 2) {
-        const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(at + 2 * i);
-        v[i] = q.x; v[i + 1] = q.y;
-    }
-}
-__device__ __forceinline__ void st_pairs(float* at, const f2 (&v)[kPairs]) {
-#pragma unroll
-    for (int i = 0; i < kPairs; i += 2) *reinterpret_cast<ulonglong2*>(at + 2 * i) = make_ulonglong2(v[i], v[i + 1]);
-}
 template <int DT>
 __device__ __forceinline__ void unpack_pairs(const Pack<DT, kPw>& r, f2 (&v)[kPairs]) {
     float f[kPw];
@@ -90,14 +136,6 @@ __device__ __forceinline__ void unpack_pairs(const Pack<DT, kPw>& r, f2 (&v)[kPa
 #pragma unroll
     for (int i = 0; i < kPairs; ++i) v[i] = f2_pack(f[2 * i], f[2 * i + 1]);
 }
-template <int DT, bool Vec>
-__device__ __forceinline__ void st_row(void* base, long long i, int valid, const f2 (&v)[kPairs]) {
-    float f[kPw];
-#pragma unroll
-    for (int c = 0; c < kPairs; ++c) f2_unpack(v[c], f[2 * c], f[2 * c + 1]);
-    st_pack<DT, kPw, Vec>(base, i, valid, f);
-}
-
 // The gate's activation and its derivative.  silu and sigmoid are one expression: s t with t = g or 1, derivative m s + s (1 - s) t
 // with m = 1 or 0.
 struct GateAct {
@@ -120,7 +158,7 @@ norm_residual_fwd_kernel(const __grid_constant__ NrP p) {
     extern __shared__ __align__(16) float weights[];
     __shared__ float red[2][32];
     put_weights(p, weights);
-    const Place at(p);
+    const Place<Vec> at(p);
     const int D = p.a.D;
     RowSum sum{red, 0, at.group * (p.per_row / 32), p.per_row / 32};
     const GateAct act(p.a.activation);
@@ -129,12 +167,11 @@ norm_residual_fwd_kernel(const __grid_constant__ NrP p) {
     Pack<DT, kPw> nx = {}, ng = {};
     Pack<RDT, kPw> nr = {};
     auto request = [&](long long row) {
-        const int ok = row < p.a.rows ? at.valid : 0;
-        if (ok <= 0 && at.rows == 1) return;                // (a thread behind the row's end keeps its zeros)
-        const long long i = row * D + at.col;
-        nx = ld_pack<DT, kPw, Vec, true>(p.a.x, i, ok);
-        if (p.a.residual) nr = ld_pack<RDT, kPw, Vec, true>(p.a.residual, i, ok);
-        if (p.a.gate) ng = ld_pack<DT, kPw, Vec, true>(p.a.gate, i, ok);
+        const bool exists = row < p.a.rows;
+        if (at.rows == 1 && !(exists && at.any())) return;      // (a thread behind the row's end keeps its zeros)
+        nx = at.template load<DT>(p.a.x, row, exists);
+        if (p.a.residual) nr = at.template load<RDT>(p.a.residual, row, exists);
+        if (p.a.gate) ng = at.template load<DT>(p.a.gate, row, exists);
     };
     long long first = (long long)blockIdx.x * at.rows;
     const long long step = (long long)gridDim.x * at.rows;
@@ -152,32 +189,31 @@ norm_residual_fwd_kernel(const __grid_constant__ NrP p) {
 #pragma unroll
             for (int c = 0; c < kPairs; ++c) ss = f2_fma(v[c], v[c], ss);
             const float factor = root * rsqrtf(sum.one(f2_sum(ss)) + p.a.eps);
-            if (p.a.factors && at.col == 0 && row < p.a.rows) p.a.factors[2 * row] = factor;
+            if (p.a.factors && at.lane == 0 && row < p.a.rows) p.a.factors[2 * row] = factor;
             const f2 k = f2_dup(factor);
-            ld_pairs(weights + at.col, w);
+            at.get(weights, w);
 #pragma unroll
             for (int c = 0; c < kPairs; ++c) v[c] = f2_mul(v[c], f2_mul(k, w[c]));
         }
         if (p.a.gate)
 #pragma unroll
             for (int c = 0; c < kPairs; ++c) v[c] = f2_mul(v[c], act.value(g[c], sigmoid_pair(g[c])));
-        ld_pairs(weights + 2 * p.stride + at.col, w);
+        at.get(weights + 2 * p.stride, w);
         f2 ss = 0;
 #pragma unroll
         for (int c = 0; c < kPairs; ++c) {
             r[c] = f2_fma(w[c], v[c], r[c]);
             ss = f2_fma(r[c], r[c], ss);
         }
-        const int ok = row < p.a.rows ? at.valid : 0;
-        st_row<RDT, Vec>(p.a.r, row * D + at.col, ok, r);
+        at.template store<RDT>(p.a.r, row, row < p.a.rows, r);
         if (p.a.pre_weight) {
             const float factor = root * rsqrtf(sum.one(f2_sum(ss)) + p.a.eps);
-            if (p.a.factors && at.col == 0 && row < p.a.rows) p.a.factors[2 * row + 1] = factor;
+            if (p.a.factors && at.lane == 0 && row < p.a.rows) p.a.factors[2 * row + 1] = factor;
             const f2 k = f2_dup(factor);
-            ld_pairs(weights + p.stride + at.col, w);
+            at.get(weights + p.stride, w);
 #pragma unroll
             for (int c = 0; c < kPairs; ++c) r[c] = f2_mul(r[c], f2_mul(k, w[c]));
-            st_row<DT, Vec>(p.a.u, row * D + at.col, ok, r);
+            at.template store<DT>(p.a.u, row, row < p.a.rows, r);
         }
     }
 }
@@ -188,17 +224,17 @@ __global__ void __launch_bounds__(MaxThreads, MaxThreads == 256 ? 2 : 1) norm_re
     __shared__ float red[2][32];
     constexpr bool Lean = MaxThreads > 512;
     put_weights(p, weights);
-    const Place at(p);
+    const Place<Vec> at(p);
     const int D = p.a.D;
     RowSum sum{red, 0, at.group * (p.per_row / 32), p.per_row / 32};
     const GateAct act(p.a.activation);
     f2 acc[Lean ? 1 : 3][kPairs];                           // post, pre, scale
-    float* sums = weights + 3 * p.stride + at.col;
+    float* sums = weights + 3 * p.stride;
 #pragma unroll
     for (int c = 0; c < kPairs; ++c) acc[0][c] = 0;
 #pragma unroll
     for (int k = 0; k < 3; ++k) {
-        if (Lean) st_pairs(sums + k * p.stride, acc[0]);
+        if (Lean) at.put(sums + k * p.stride, acc[0]);
         else
 #pragma unroll
             for (int c = 0; c < kPairs; ++c) acc[Lean ? 0 : k][c] = 0;
@@ -206,10 +242,10 @@ __global__ void __launch_bounds__(MaxThreads, MaxThreads == 256 ? 2 : 1) norm_re
     auto add = [&](int k, const f2 (&a)[kPairs], const f2 (&b)[kPairs]) {      // sum k += a b
         if constexpr (Lean) {
             f2 t[kPairs];
-            ld_pairs(sums + k * p.stride, t);
+            at.get(sums + k * p.stride, t);
 #pragma unroll
             for (int c = 0; c < kPairs; ++c) t[c] = f2_fma(a[c], b[c], t[c]);
-            st_pairs(sums + k * p.stride, t);
+            at.put(sums + k * p.stride, t);
         } else {
 #pragma unroll
             for (int c = 0; c < kPairs; ++c) acc[k][c] = f2_fma(a[c], b[c], acc[k][c]);
@@ -225,14 +261,13 @@ __global__ void __launch_bounds__(MaxThreads, MaxThreads == 256 ? 2 : 1) norm_re
     Pack<DT, kPw> nx = {}, ng = {}, nu = {};
     Pack<RDT, kPw> nr = {}, nd = {};
     auto request = [&](long long row) {
-        const int ok = row < p.a.rows ? at.valid : 0;
-        if (ok <= 0 && at.rows == 1) return;                // (a thread behind the row's end keeps its zeros)
-        const long long i = row * D + at.col;
-        nx = ld_pack<DT, kPw, Vec, true>(p.a.x, i, ok);
-        if (p.a.residual) nr = ld_pack<RDT, kPw, Vec, true>(p.a.residual, i, ok);
-        if (p.a.gate) ng = ld_pack<DT, kPw, Vec, true>(p.a.gate, i, ok);
-        if (p.a.dr) nd = ld_pack<RDT, kPw, Vec, true>(p.a.dr, i, ok);
-        if (p.a.du) nu = ld_pack<DT, kPw, Vec, true>(p.a.du, i, ok);
+        const bool exists = row < p.a.rows;
+        if (at.rows == 1 && !(exists && at.any())) return;      // (a thread behind the row's end keeps its zeros)
+        nx = at.template load<DT>(p.a.x, row, exists);
+        if (p.a.residual) nr = at.template load<RDT>(p.a.residual, row, exists);
+        if (p.a.gate) ng = at.template load<DT>(p.a.gate, row, exists);
+        if (p.a.dr) nd = at.template load<RDT>(p.a.dr, row, exists);
+        if (p.a.du) nu = at.template load<DT>(p.a.du, row, exists);
     };
     long long first = (long long)blockIdx.x * at.rows;
     const long long step = (long long)gridDim.x * at.rows;
@@ -259,7 +294,7 @@ __global__ void __launch_bounds__(MaxThreads, MaxThreads == 256 ? 2 : 1) norm_re
         if (p.a.pre_weight) {
             f2 x[kPairs], r[kPairs], w[kPairs], k[kPairs], dot = 0;
             unpack_pairs<DT>(cx, x);
-            ld_pairs(weights + at.col, w);
+            at.get(weights, w);
 #pragma unroll
             for (int c = 0; c < kPairs; ++c) x[c] = f2_mul(x[c], f2_mul(w[c], f2_dup(kx)));
             if (p.a.gate) {
@@ -269,8 +304,8 @@ __global__ void __launch_bounds__(MaxThreads, MaxThreads == 256 ? 2 : 1) norm_re
                 for (int c = 0; c < kPairs; ++c) x[c] = f2_mul(x[c], act.value(g[c], s[c]));
             }
             unpack_pairs<RDT>(cr, r);
-            ld_pairs(weights + 2 * p.stride + at.col, k);
-            ld_pairs(weights + p.stride + at.col, w);
+            at.get(weights + 2 * p.stride, k);
+            at.get(weights + p.stride, w);
             f2 t[kPairs];
             unpack_pairs<DT>(cu, t);
 #pragma unroll
@@ -286,17 +321,15 @@ __global__ void __launch_bounds__(MaxThreads, MaxThreads == 256 ? 2 : 1) norm_re
             }
             add(1, t, r);
         }
-        const int ok = exists ? at.valid : 0;
-        const long long i = row * D + at.col;
-        if (p.a.dresidual) st_row<RDT, Vec>(p.a.dresidual, i, ok, d);
+        if (p.a.dresidual) at.template store<RDT>(p.a.dresidual, row, exists, d);
         f2 x[kPairs], w[kPairs];
         unpack_pairs<DT>(cx, x);
-        ld_pairs(weights + at.col, w);
+        at.get(weights, w);
         {
             f2 n[kPairs], k[kPairs];
 #pragma unroll
             for (int c = 0; c < kPairs; ++c) n[c] = f2_mul(x[c], f2_mul(w[c], f2_dup(kx)));
-            ld_pairs(weights + 2 * p.stride + at.col, k);
+            at.get(weights + 2 * p.stride, k);
             if (p.a.gate) {
                 f2 g[kPairs], v[kPairs];
                 unpack_pairs<DT>(cg, g);
@@ -308,7 +341,7 @@ __global__ void __launch_bounds__(MaxThreads, MaxThreads == 256 ? 2 : 1) norm_re
                     k[c] = f2_mul(dv, a);
                 }
                 add(2, d, v);
-                if (p.a.dgate) st_row<DT, Vec>(p.a.dgate, i, ok, g);
+                if (p.a.dgate) at.template store<DT>(p.a.dgate, row, exists, g);
             } else {
                 add(2, d, n);
 #pragma unroll
@@ -328,7 +361,7 @@ __global__ void __launch_bounds__(MaxThreads, MaxThreads == 256 ? 2 : 1) norm_re
 #pragma unroll
             for (int c = 0; c < kPairs; ++c) d[c] = f2_fma(d[c], w[c], f2_mul(f2_dup(-back), x[c]));
         }
-        st_row<DT, Vec>(p.a.dx, i, ok, d);
+        at.template store<DT>(p.a.dx, row, exists, d);
     }
 #pragma unroll
     for (int k = 0; k < 3; ++k) {
@@ -337,7 +370,7 @@ __global__ void __launch_bounds__(MaxThreads, MaxThreads == 256 ? 2 : 1) norm_re
         if (Lean) {
             for (int c = threadIdx.x; c < D; c += blockDim.x) to[c] = weights[(3 + k) * p.stride + c];
         } else {
-            st_pairs(weights + at.group * p.stride + at.col, acc[Lean ? 0 : k]);
+            at.put(weights + at.group * p.stride, acc[Lean ? 0 : k]);
             __syncthreads();
             for (int c = threadIdx.x; c < D; c += blockDim.x) {
                 float v = 0.f;
