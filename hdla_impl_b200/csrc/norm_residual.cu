@@ -8,10 +8,12 @@
 // of 256 threads fit on an SM: with them in registers backward had one, and took 686 instead of 319 us for 32768 rows of 2048.
 // Backward computes r again from the inputs in fp32 (as many bytes as reading the rounded r), reads the norms' factors that
 // forward left (305 -> 276 us: a sum and a barrier less), takes the two sums that remain (the dot products of the norms'
-// gradients), and keeps the sums over rows (gradients of the weights and of scale) in registers until its last row; blocks'
-// sums are added in a fixed order.  Rows of more than 4096 channels need 1024 threads of 64 registers: there those sums are in
-// shared memory too, and nothing is requested ahead.  32768 rows of 2048, bf16, all parts: forward 131 us = 5.1 TB/s (0.80 of
-// the measured copy), backward 271 us = 4.0 TB/s (0.61); what backward waits for is the chain of its two sums.
+// gradients; the row that such a product belongs to is normed before the two meet, since the cube of a norm's factor need not be
+// an fp32 number where the gradient is one, as for rows of 1e12 or of 1e-14), and keeps the sums over rows (gradients of the
+// weights and of scale) in registers until its last row; blocks' sums are added in a fixed order.  Rows of more than 4096
+// channels need 1024 threads of 64 registers: there those sums are in shared memory too, and nothing is requested ahead.
+// 32768 rows of 2048, bf16, all parts: forward 131 us = 5.1 TB/s (0.80 of the measured copy), backward 271 us = 4.0 TB/s
+// (0.61); what backward waits for is the chain of its two sums.
 #include "ssm.cuh"
 
 namespace hdla {
@@ -313,11 +315,11 @@ __global__ void __launch_bounds__(MaxThreads, MaxThreads == 256 ? 2 : 1) norm_re
                 r[c] = f2_fma(k[c], x[c], r[c]);
                 dot = f2_fma(f2_mul(t[c], w[c]), r[c], dot);
             }
-            const float back = kr * kr * kr * per * sum.one(f2_sum(dot));
+            const float back = kr * (kr * per * sum.one(f2_sum(dot)));
 #pragma unroll
             for (int c = 0; c < kPairs; ++c) {
-                t[c] = f2_mul(t[c], f2_dup(kr));
-                d[c] = f2_fma(t[c], w[c], f2_fma(f2_dup(-back), r[c], d[c]));
+                r[c] = f2_mul(r[c], f2_dup(kr));
+                d[c] = f2_fma(f2_mul(t[c], f2_dup(kr)), w[c], f2_fma(f2_dup(-back), r[c], d[c]));
             }
             add(1, t, r);
         }
@@ -354,12 +356,12 @@ __global__ void __launch_bounds__(MaxThreads, MaxThreads == 256 ? 2 : 1) norm_re
             f2 dot = 0;
 #pragma unroll
             for (int c = 0; c < kPairs; ++c) dot = f2_fma(f2_mul(d[c], w[c]), x[c], dot);
-            const float back = kx * kx * kx * per * sum.one(f2_sum(dot));
+            const float back = kx * (kx * per * sum.one(f2_sum(dot)));
 #pragma unroll
-            for (int c = 0; c < kPairs; ++c) d[c] = f2_mul(d[c], f2_dup(kx));
+            for (int c = 0; c < kPairs; ++c) x[c] = f2_mul(x[c], f2_dup(kx));
             add(0, d, x);
 #pragma unroll
-            for (int c = 0; c < kPairs; ++c) d[c] = f2_fma(d[c], w[c], f2_mul(f2_dup(-back), x[c]));
+            for (int c = 0; c < kPairs; ++c) d[c] = f2_fma(f2_mul(d[c], f2_dup(kx)), w[c], f2_mul(f2_dup(-back), x[c]));
         }
         at.template store<DT>(p.a.dx, row, exists, d);
     }

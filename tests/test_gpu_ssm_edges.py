@@ -1,0 +1,54 @@
+"""GPU: calls of the short convolution, the selective scan and the norms round a block that lie at the edge of what they take.
+
+Tolerances are of the kind of test_gpu_ssm.py: an output of type t is rounded once (finfo(t).eps / 2), all else is fp32."""
+import math
+
+import pytest
+import torch
+
+from oracle import ssm_oracle as orc
+
+pytestmark = pytest.mark.gpu
+BF, F32 = torch.bfloat16, torch.float32
+
+
+@pytest.fixture(scope="module")
+def dev():
+    assert torch.cuda.is_available(), "these tests need a CUDA device"
+    return torch.device("cuda:0")
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def rn(g, *s, dtype=F32, scale=1.0):
+    return (scale * torch.randn(*s, generator=g)).to(dtype)
+
+
+def off(got, ref):
+    """Largest difference relative to the largest value of the definition."""
+    assert got.shape == ref.shape and bool(torch.isfinite(got).all())
+    return float((got.detach().cpu().double() - ref.detach()).abs().max()) / float(ref.detach().abs().max())
+
+
+# --------------------------------------------------------------------------------------------- norms
+@pytest.mark.parametrize("D", [64, 1001, 8192])
+@pytest.mark.parametrize("which", ["post_weight", "pre_weight"])
+@pytest.mark.parametrize("size,eps", [(1e12, 1e-5), (1e15, 1e-5), (1e-14, 1e-30)])
+def test_norms_of_large_and_of_tiny_rows(dev, D, which, size, eps):
+    """The norms' gradient takes its second term, the projection on the row, where the cube of the norm's factor is no fp32 number
+    (1e-45 at rows of 1e15, 1e42 at rows of 1e-14), and so do the gradients that are small themselves (dy of 1e-3)."""
+    from hdla_impl_b200 import layer_ops
+    g = gen(D)
+    x, w, do = rn(g, 3, D, scale=size), rn(g, D), rn(g, 3, D, scale=1e-3)
+    a, v = x.to(dev).requires_grad_(True), w.to(dev).requires_grad_(True)
+    y = [t for t in layer_ops.rms_norm_residual(a, **{which: v}, eps=eps) if t is not None][-1]
+    got = torch.autograd.grad(y, [a, v], do.to(dev))
+    b, c = x.double().requires_grad_(True), w.double().requires_grad_(True)
+    r = [t for t in orc.norm_residual(b, **{which[:-7]: c}, eps=eps) if t is not None][-1]
+    # sums of D roundings of random sign and a dozen operations: (sqrt(D) + 64) 2^-21, and the gradient is a difference: 8 times
+    tol = 8 * (math.sqrt(D) + 64) * 2.0 ** -21
+    assert off(y, r) <= tol
+    for p, q in zip(got, torch.autograd.grad(r, [b, c], do.double())):
+        assert off(p, q) <= tol
