@@ -44,6 +44,12 @@ Tensor space(size_t bytes, const Tensor& like) {
     return bytes ? dense({static_cast<int64_t>(bytes)}, at::kByte, like.device()) : Tensor();
 }
 Tensor as_type(const Tensor& t, at::ScalarType st) { return t.defined() && t.scalar_type() != st ? t.to(st) : t; }
+// The type that weights used together have in a kernel: the widest among them (all products and sums are fp32 either way).
+at::ScalarType weights_type(std::initializer_list<const Tensor*> ts) {
+    for (const Tensor* t : ts)
+        if (t->defined() && t->scalar_type() != at::kBFloat16) return at::kFloat;
+    return at::kBFloat16;
+}
 Tensor grad_in(const Tensor& g, at::ScalarType st) { return g.defined() ? g.to(st).contiguous() : g; }
 bool is_float(const Tensor& t) { return !t.defined() || t.is_floating_point(); }
 bool shape3(const Tensor& t, int64_t a, int64_t b, int64_t c) { return t.dim() == 3 && t.size(0) == a && t.size(1) == b && t.size(2) == c; }
@@ -63,7 +69,7 @@ Tensor unpack_saved(const Saved& s, const char* node) {
 }
 
 // ------------------------------------------------------------------------------------------ short convolution
-struct ConvIn { Tensor x, w, b, h0, cu; bool silu = false; };
+struct ConvIn { Tensor x, w, b, h0, cu; bool silu = false; };      // (w and b of one type)
 
 HdlaConvArgs conv_args(const ConvIn& i) {
     HdlaConvArgs a{};
@@ -105,7 +111,7 @@ ConvGrads conv_backward(const ConvIn& i, const Tensor& dy_, const Tensor& dht_) 
 struct ConvNode : torch::autograd::Node {
     Saved x, w, b, h0, cu;
     bool silu = false;
-    at::ScalarType b_type = at::kFloat;
+    at::ScalarType w_type = at::kFloat, b_type = at::kFloat;
     std::string name() const override { return "HdlaShortConvBackward"; }
     void release_variables() override {
         std::lock_guard<std::mutex> lock(mutex_);
@@ -118,9 +124,14 @@ struct ConvNode : torch::autograd::Node {
         if (!grads[0].defined() && !dht.defined()) return variable_list(4);
         const char* me = "HdlaShortConvBackward";
         ConvGrads g = conv_backward({unpack_saved(x, me), w.get(me), b.get(me), h0.get(me), cu.get(me), silu}, grads[0], dht);
-        return {g.dx, g.dw, as_type(g.db, b_type), g.dh0};
+        return {g.dx, as_type(g.dw, w_type), as_type(g.db, b_type), g.dh0};
     }
 };
+
+ConvIn conv_in(const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& h0, const Tensor& cu, bool silu) {
+    const auto type = weights_type({&w, &b});
+    return {rows_of(x), as_type(w, type).contiguous(), b.defined() ? as_type(b, type).contiguous() : b, h0.defined() ? h0.contiguous() : h0, cu, silu};
+}
 
 std::pair<Tensor, Tensor> conv_op(const Tensor& x_, const Tensor& w_, const Tensor& b_, const Tensor& h0_, const Tensor& cu, bool silu, bool want_ht) {
     const bool grad = needs_grad({&x_, &w_, &b_, &h0_});
@@ -129,13 +140,13 @@ std::pair<Tensor, Tensor> conv_op(const Tensor& x_, const Tensor& w_, const Tens
     {
         at::NoGradGuard no_grad;
         c10::cuda::CUDAGuard guard(x_.device());
-        const ConvIn i{rows_of(x_), w_.contiguous(), b_.defined() ? as_type(b_, w_.scalar_type()).contiguous() : b_,
-                       h0_.defined() ? h0_.contiguous() : h0_, cu, silu};
+        const ConvIn i = conv_in(x_, w_, b_, h0_, cu, silu);
         r = conv_forward(i, want_ht);
         if (grad) {
             node = make_node<ConvNode>();
             node->x.save(i.x); node->w.save(i.w); node->b.save(i.b); node->h0.save(i.h0); node->cu.save(i.cu);
             node->silu = silu;
+            node->w_type = w_.scalar_type();
             if (b_.defined()) node->b_type = b_.scalar_type();
         }
     }
@@ -187,8 +198,8 @@ PyObject* py_short_conv_backward(PyObject*, PyObject* const* av, Py_ssize_t n) {
     if (!guarded([&] {
             at::NoGradGuard no_grad;
             c10::cuda::CUDAGuard guard(c.x->device());
-            g = conv_backward({rows_of(*c.x), c.w->contiguous(), c.b->defined() ? as_type(*c.b, c.w->scalar_type()).contiguous() : *c.b,
-                               c.h0->defined() ? c.h0->contiguous() : *c.h0, *c.cu, c.silu}, *dy, *dht);
+            g = conv_backward(conv_in(*c.x, *c.w, *c.b, *c.h0, *c.cu, c.silu), *dy, *dht);
+            g.dw = as_type(g.dw, c.w->scalar_type());
             if (g.db.defined()) g.db = as_type(g.db, c.b->scalar_type());
         }))
         return nullptr;
@@ -210,7 +221,8 @@ PyObject* py_short_conv_step(PyObject*, PyObject* const* av, Py_ssize_t n) {
     if (!guarded([&] {
             at::NoGradGuard no_grad;
             c10::cuda::CUDAGuard guard(x->device());
-            const Tensor xr = rows_of(*x), wc = w->contiguous(), bc = b->defined() ? as_type(*b, w->scalar_type()).contiguous() : *b;
+            const auto type = weights_type({w, b});
+            const Tensor xr = rows_of(*x), wc = as_type(*w, type).contiguous(), bc = b->defined() ? as_type(*b, type).contiguous() : *b;
             HdlaConvArgs a{};                                  // (filled in here: views of one token cost more than the call)
             a.B = (int)B; a.T = 1; a.D = (int)D; a.W = (int)W;
             a.dtype = dtype_code(xr); a.w_dtype = dtype_code(wc); a.activation = silu ? HDLA_ACT_SILU : HDLA_ACT_NONE;
@@ -490,10 +502,7 @@ NormGrads norm_backward(const NormIn& i, const Tensor& factors, const Tensor& dr
 struct NormCall { const Tensor *x, *r, *g, *scale, *post, *pre; double scale_value, eps; int act; };
 NormIn norm_in(const NormCall& c) {
     NormIn i;
-    // the weights share a type: the widest among them (a sum of products in fp32 either way)
-    bool bf = true;
-    for (const Tensor* t : {c.post, c.pre, c.scale}) bf = bf && (!t->defined() || t->scalar_type() == at::kBFloat16);
-    i.w_type = bf ? at::kBFloat16 : at::kFloat;
+    i.w_type = weights_type({c.post, c.pre, c.scale});
     auto weight = [&](const Tensor& t) { return t.defined() ? as_type(t, i.w_type).contiguous() : t; };
     i.x = c.x->contiguous(); i.r = c.r->defined() ? c.r->contiguous() : *c.r; i.g = c.g->defined() ? c.g->contiguous() : *c.g;
     i.post = weight(*c.post); i.pre = weight(*c.pre); i.scale = weight(*c.scale);

@@ -184,7 +184,7 @@ def short_convolution(
 ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """Depthwise causal convolution: ``y_t = act(bias + sum_{k<W} weight[:, W-1-k] x_{t-k})`` for W of 1 to 8 taps.  The rows
     before a sequence come from ``initial_state`` (its last row the most recent) or are zero; the final state is the last W-1 rows
-    of (initial state, x).  With ``cu_seqlens`` B is 1 and n the number of sequences; rows behind the last offset give zeros."""
+    of (initial state, x).  Weight and bias may be of other types than x; each is used as it is, in fp32 arithmetic.  With ``cu_seqlens`` B is 1 and n the number of sequences; rows behind the last offset give zeros."""
     silu = _silu(activation)
     cu = _offsets(cu_seqlens, x)
     r = (_lib._native or _lib.native()).short_conv(x, weight, bias, silu, initial_state, cu, output_final_state)

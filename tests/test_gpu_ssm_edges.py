@@ -52,3 +52,27 @@ def test_norms_of_large_and_of_tiny_rows(dev, D, which, size, eps):
     assert off(y, r) <= tol
     for p, q in zip(got, torch.autograd.grad(r, [b, c], do.double())):
         assert off(p, q) <= tol
+
+
+# --------------------------------------------------------------------------------------------- short convolution
+@pytest.mark.parametrize("xt", [F32, BF])
+@pytest.mark.parametrize("wt,bt", [(BF, F32), (F32, BF), (BF, torch.float16), (BF, torch.float64)])
+def test_taps_and_bias_of_different_types_keep_their_digits(dev, xt, wt, bt):
+    """The wider of the two is not rounded to the other's type: prompts, gradients and single tokens."""
+    from hdla_impl_b200 import ssm
+    g = gen(4)
+    x, w, b, do = rn(g, 2, 40, 16, dtype=xt), rn(g, 16, 4, dtype=wt), rn(g, 16, scale=50).to(bt), rn(g, 2, 40, 16, dtype=xt)
+    h0 = torch.zeros(2, 3, 16, dtype=xt)
+    t = [v.to(dev).requires_grad_(True) for v in (x, w, b)]
+    y, _ = ssm.short_convolution(*t, activation=None)
+    got = torch.autograd.grad(y, t, do.to(dev))
+    with torch.no_grad():
+        first = ssm.short_convolution_step(t[0][:, 0], h0.to(dev), *t[1:], activation=None)
+    assert torch.equal(first, y[:, 0])
+    ref = [v.double().requires_grad_(True) for v in (x, w, b)]
+    r, _ = orc.short_conv(*ref, None)
+    half = lambda t: torch.finfo(t).eps / 2  # noqa: E731
+    # five roundings of fp32 a sum of taps, one to the output's type; the weights' gradients are sums of 80 terms
+    assert off(y, r) <= half(xt) + 64 * 2.0 ** -24
+    for a, v, q in zip(got, t, torch.autograd.grad(r, ref, do.double())):
+        assert a.dtype == v.dtype and off(a, q) <= half(max(a.dtype, F32, key=lambda d: torch.finfo(d).eps)) + 80 * 2.0 ** -24
