@@ -15,6 +15,7 @@
 // and F come from a first kernel that runs the recurrence alone, from zero; the second kernel's blocks chain the maps of
 // the segments before theirs.
 #pragma once
+#include "lane_sums.cuh"
 #include "ssm.cuh"
 
 namespace hdla {
@@ -110,18 +111,6 @@ __device__ __forceinline__ void scatter_sum(float (&v)[N], int lane, int low) {
         }
     }
 }
-template <int N, int M>
-__device__ __forceinline__ int scatter_at(int lane, int low) {
-    int n = N, at = 0;
-#pragma unroll
-    for (int m = 1; m < M; m <<= 1)
-        if (n > 1) {
-            n >>= 1;
-            if (lane & (m * low)) at += n;
-        }
-    return at;
-}
-
 // four states of one channel (state 0 of the channel at `at`, this lane's first at n0), zero beyond N
 __device__ __forceinline__ void ld_state(const float* at, int n0, int N, bool vec, f2 (&h)[2]) {
     float v[4] = {0.f, 0.f, 0.f, 0.f};

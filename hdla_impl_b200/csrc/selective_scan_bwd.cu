@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(kScanThreads, Maps ? 5 : 3) scan_bwd_kernel(co
             float v[4];
             unpair(sum, v);
             scatter_sum<4, Parts>(v, w.lane, NL);
-            if (o + out_tok < tokens)
+            if (o + out_tok < tokens && scatter_owner<4, Parts>(w.lane, NL))
 #pragma unroll
                 for (int i = 0; i < (Parts < 4 ? 4 / Parts : 1); ++i) {
                     float* to = share + o * share_token + which * NP + i;

@@ -76,3 +76,31 @@ def test_taps_and_bias_of_different_types_keep_their_digits(dev, xt, wt, bt):
     assert off(y, r) <= half(xt) + 64 * 2.0 ** -24
     for a, v, q in zip(got, t, torch.autograd.grad(r, ref, do.double())):
         assert a.dtype == v.dtype and off(a, q) <= half(max(a.dtype, F32, key=lambda d: torch.finfo(d).eps)) + 80 * 2.0 ** -24
+
+
+# --------------------------------------------------------------------------------------------- selective scan
+def test_shares_of_few_states_take_turns(dev):
+    """Eight states, sixteen groups of 68 channels (two tiles of channels each), 2^23 tokens times groups: one tile's shares of dB and
+    dC take half of the limit of 1 GiB and a little more, so that the tiles of the whole batch go in two launches, the second of which
+    adds to the first's shares; those of each row of the batch go in one.  Decays of a half and less a token: what a row's cuts into
+    segments round differently is as small as a state's own rounding."""
+    from hdla_impl_b200 import ssm
+    G, per, N, T = 16, 68, 8, (1 << 18) + 8
+    D = G * per
+    g = torch.Generator(device=dev).manual_seed(17)
+    rnd = lambda *s: torch.randn(*s, generator=g, device=dev, dtype=BF)  # noqa: E731
+    t = {"x": rnd(2, T, D), "dt": rnd(2, T, D).abs_(), "B": rnd(2, T, G, N), "C": rnd(2, T, G, N)}
+    A = -1 - torch.rand(D, N, generator=g, device=dev)
+    dy = rnd(2, T, D)
+
+    def f(rows):
+        leaves = [v[rows].detach().requires_grad_(k in "BC") for k, v in t.items()]
+        y, _ = ssm.selective_scan(leaves[0], leaves[1], A, *leaves[2:])
+        return torch.autograd.grad(y, leaves[2:], dy[rows])
+
+    whole = f(slice(0, 2))
+    for b in range(2):
+        for name, a, c in zip(("dB", "dC"), whole, f(slice(b, b + 1))):
+            # both sides are rounded to bf16; fp32 before that, over a state's memory of some ten tokens and 68 channels
+            e = float((a[b].float() - c[0].float()).abs().max() / c.float().abs().max())
+            assert e <= 2 * torch.finfo(BF).eps / 2 + 128 * 2.0 ** -21, (name, b, e)
