@@ -387,6 +387,9 @@ __global__ void __launch_bounds__(MaxThreads, MaxThreads == 256 ? 2 : 1) norm_re
 int row_threads(int D) { return ((D + kPw - 1) / kPw + 31) / 32 * 32; }
 int block_threads(int per_row) { return per_row >= 256 ? per_row : 256 / per_row * per_row; }
 
+// the threads that a kernel for blocks of `threads` is built for
+int built_for(int threads) { return threads > 512 ? 1024 : threads > 256 ? 512 : 256; }
+
 bool norm_vec(const HdlaNormResidualArgs& a) {
     for (const void* q : {a.x, a.residual, a.gate, (const void*)a.r, (const void*)a.u, a.dr, a.du, (const void*)a.dx,
                           (const void*)a.dresidual, (const void*)a.dgate})
@@ -397,8 +400,12 @@ bool norm_vec(const HdlaNormResidualArgs& a) {
 typedef void (*Kernel)(const NrP);
 template <int DT, int RDT, bool Vec>
 Kernel kernel_for(bool backward, int threads) {
-    if (backward) return threads > 512 ? norm_residual_bwd_kernel<DT, RDT, Vec, 1024> : threads > 256 ? norm_residual_bwd_kernel<DT, RDT, Vec, 512> : norm_residual_bwd_kernel<DT, RDT, Vec, 256>;
-    return threads > 512 ? norm_residual_fwd_kernel<DT, RDT, Vec, 1024> : threads > 256 ? norm_residual_fwd_kernel<DT, RDT, Vec, 512> : norm_residual_fwd_kernel<DT, RDT, Vec, 256>;
+    const int n = built_for(threads);
+    if (backward)
+        return n == 1024 ? norm_residual_bwd_kernel<DT, RDT, Vec, 1024> : n == 512 ? norm_residual_bwd_kernel<DT, RDT, Vec, 512>
+                                                                                    : norm_residual_bwd_kernel<DT, RDT, Vec, 256>;
+    return n == 1024 ? norm_residual_fwd_kernel<DT, RDT, Vec, 1024> : n == 512 ? norm_residual_fwd_kernel<DT, RDT, Vec, 512>
+                                                                                : norm_residual_fwd_kernel<DT, RDT, Vec, 256>;
 }
 Kernel pick(const HdlaNormResidualArgs& a, bool backward, int threads) {
     const bool vec = norm_vec(a);
@@ -424,7 +431,10 @@ int launch(const HdlaNormResidualArgs& a, bool backward, float* part, cudaStream
     const Kernel kernel = pick(a, backward, threads);
     const size_t bytes = shared_of(per_row, threads, backward);
     if (bytes > 47 << 10) {                                      // (the sums have some of the 48 KB that need no request)
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+        // The limit is the kernel's, not this launch's, and other threads may be between setting it and launching: what all of
+        // them set is the most that any launch of this kernel takes.
+        const int most = built_for(threads);
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared_of(most, most, backward));
         if (e != cudaSuccess) return fail(HDLA_ERR_CUDA, "norm_residual: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
     }
     kernel<<<blocks_of(a, backward), threads, bytes, st>>>(p);

@@ -54,6 +54,43 @@ def test_norms_of_large_and_of_tiny_rows(dev, D, which, size, eps):
         assert off(p, q) <= tol
 
 
+@pytest.mark.parametrize("D", [(4104, 8192), (2056, 4096)])
+def test_threads_with_rows_of_different_widths(dev, D):
+    """Two threads, each with its stream: widths that one kernel serves with different amounts of shared memory, forward and
+    backward.  No launch is refused, and both get what they get alone."""
+    import threading
+    from hdla_impl_b200 import layer_ops
+
+    def call(x, w):
+        x, w = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
+        r, u = layer_ops.rms_norm_residual(x, post_weight=w, pre_weight=w)
+        return [r.detach(), u.detach(), *torch.autograd.grad([r, u], [x, w], [x.detach(), x.detach()])]
+
+    g = gen(6)
+    inputs = [(rn(g, 4, d).to(dev), rn(g, d).to(dev)) for d in D]
+    want = [call(*i) for i in inputs]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(k):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream(dev)):
+                for i in range(1500):
+                    got = call(*inputs[k])
+                    if i % 100 == 0 and not all(torch.equal(a, b) for a, b in zip(got, want[k])):
+                        wrong.append((D[k], i, "values"))
+        except Exception as e:  # noqa: BLE001
+            wrong.append((D[k], repr(e)))
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not wrong, wrong
+
+
 # --------------------------------------------------------------------------------------------- short convolution
 @pytest.mark.parametrize("xt", [F32, BF])
 @pytest.mark.parametrize("wt,bt", [(BF, F32), (F32, BF), (BF, torch.float16), (BF, torch.float64)])
