@@ -174,15 +174,26 @@ bool conv_call(PyObject* const* av, ConvCall& c) {
     return same_device(x, {c.w, c.b, c.h0, c.cu});
 }
 
-// short_conv(x, weight, bias or None, silu, h0 or None, cu_seqlens or None, output_final_state) -> (y, final state or None)
+// short_conv(x, weight, bias or None, silu, h0 or None, cu_seqlens or None, output_final_state, bare) -> (y, final state or None);
+// bare: without a graph, which the Python autograd function makes
 PyObject* py_short_conv(PyObject*, PyObject* const* av, Py_ssize_t n) {
-    if (n != 7) { PyErr_SetString(PyExc_TypeError, "short_conv takes 7 arguments"); return nullptr; }
+    if (n != 8) { PyErr_SetString(PyExc_TypeError, "short_conv takes 8 arguments"); return nullptr; }
     ConvCall c;
+    const bool bare = av[7] == Py_True;
     const int want = PyObject_IsTrue(av[6]);
     if (want < 0) { PyErr_Clear(); NOT_MINE(); }
-    if (tracing() || !conv_call(av, c)) NOT_MINE();
+    if ((!bare && tracing()) || !conv_call(av, c)) NOT_MINE();
     std::pair<Tensor, Tensor> r;
-    if (!guarded([&] { r = conv_op(*c.x, *c.w, *c.b, *c.h0, *c.cu, c.silu, want); })) return nullptr;
+    if (!guarded([&] {
+            if (bare) {
+                at::NoGradGuard no_grad;
+                c10::cuda::CUDAGuard guard(c.x->device());
+                r = conv_forward(conv_in(*c.x, *c.w, *c.b, *c.h0, *c.cu, c.silu), want);
+            } else {
+                r = conv_op(*c.x, *c.w, *c.b, *c.h0, *c.cu, c.silu, want);
+            }
+        }))
+        return nullptr;
     return tuple_of({&r.first, &r.second});
 }
 // short_conv_backward(x, weight, bias, silu, h0, cu_seqlens, dy or None, dht or None) -> (dx, dweight, dbias, dh0)

@@ -17,6 +17,7 @@ the steps go on with:
 Inputs that are slices of a wider projection (dense along their last dimension) are read where they are.  Under CUDA graph
 capture give ``cu_seqlens`` as an int64 tensor on the GPU; then nothing is copied or waited for, and a replay goes by what the
 tensor then holds.  Rows behind the last offset may hold anything.  The gradients have no graph of their own (no double backward).
+``torch.jit.trace`` records the operators for whole sequences as calls; the steps refuse to be traced.
 """
 from __future__ import annotations
 
@@ -110,7 +111,10 @@ def _check_scan(x, dt, A, B, C, D, z, dt_bias, state, n) -> None:
     _need_type(all(t is None or t.is_floating_point() for t in (A, D, dt_bias, state)), "A, D, dt_bias and states must be floating-point tensors")
 
 
-def _no_grad_needed(*tensors) -> None:
+def _a_step_can_be_taken(*tensors) -> None:
+    if torch.jit.is_tracing():
+        raise RuntimeError("single-token steps update their state in place, which a trace would not record: they cannot be traced "
+                           "with torch.jit.trace")
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError("single-token steps update their state in place and have no backward; use the operator for whole "
                            "sequences, or torch.no_grad()")
@@ -125,7 +129,7 @@ class _ShortConv(torch.autograd.Function):
     def forward(ctx, x, weight, bias, silu, h0, cu, want):
         ctx.silu = silu
         ctx.save_for_backward(x, weight, bias, h0, cu)
-        r = _lib.native().short_conv(*[_plain(t) for t in (x, weight, bias)], silu, _plain(h0), _plain(cu), want)
+        r = _lib.native().short_conv(*[_plain(t) for t in (x, weight, bias)], silu, _plain(h0), _plain(cu), want, True)
         if r is NotImplemented:
             raise TypeError("short_convolution: unsupported arguments")
         return r
@@ -187,7 +191,7 @@ def short_convolution(
     of (initial state, x).  Weight and bias may be of other types than x; each is used as it is, in fp32 arithmetic.  With ``cu_seqlens`` B is 1 and n the number of sequences; rows behind the last offset give zeros."""
     silu = _silu(activation)
     cu = _offsets(cu_seqlens, x)
-    r = (_lib._native or _lib.native()).short_conv(x, weight, bias, silu, initial_state, cu, output_final_state)
+    r = (_lib._native or _lib.native()).short_conv(x, weight, bias, silu, initial_state, cu, output_final_state, False)
     if r is not NotImplemented:
         return r
     _need(x.dim() == 3, f"x must have 3 dimensions [B, T, D], got {x.dim()}")
@@ -210,7 +214,7 @@ def short_convolution_step(
     _need(x.dim() == 2, f"x must have 2 dimensions [B, D], got {x.dim()}")
     _check_conv(x, weight, bias, activation, state, x.shape[0], 2)
     _need(state.is_contiguous(), "the state is updated in place: it must be contiguous")
-    _no_grad_needed(x, state, weight, bias)
+    _a_step_can_be_taken(x, state, weight, bias)
     r = _lib.native().short_conv_step(*[_plain(t) for t in (x, state, weight, bias)], silu)
     if r is NotImplemented:
         raise TypeError("short_convolution_step: unsupported arguments")
@@ -266,7 +270,7 @@ def selective_scan_step(
     _need(x.dim() == 2, f"x must have 2 dimensions [B, D], got {x.dim()}")
     _check_scan(x, dt, A, B, C, D, z, dt_bias, state, x.shape[0])
     _need(state.dtype == torch.float32 and state.is_contiguous(), "the state is updated in place: it must be contiguous and float32")
-    _no_grad_needed(x, dt, A, B, C, D, z, dt_bias, state)
+    _a_step_can_be_taken(x, dt, A, B, C, D, z, dt_bias, state)
     r = _lib.native().selective_scan_step(*[_plain(t) for t in (x, dt, A, B, C, D, z, dt_bias)], softplus, _plain(state))
     if r is NotImplemented:
         raise TypeError("selective_scan_step: unsupported arguments")

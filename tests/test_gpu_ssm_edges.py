@@ -141,3 +141,42 @@ def test_shares_of_few_states_take_turns(dev):
             # both sides are rounded to bf16; fp32 before that, over a state's memory of some ten tokens and 68 channels
             e = float((a[b].float() - c[0].float()).abs().max() / c.float().abs().max())
             assert e <= 2 * torch.finfo(BF).eps / 2 + 128 * 2.0 ** -21, (name, b, e)
+
+
+# --------------------------------------------------------------------------------------------- tracing
+def traceable(dev):
+    """{name: (function of tensors, tensors)}: each operator for whole sequences."""
+    from hdla_impl_b200 import layer_ops, ssm
+    g = gen(23)
+    D, N = 24, 8
+    x, z, w, b = rn(g, 2, 30, D, dtype=BF), rn(g, 2, 30, D, dtype=BF), rn(g, D, 4, dtype=BF), rn(g, D, dtype=BF)
+    bc, A = rn(g, 2, 30, N, dtype=BF), -torch.exp(rn(g, D, N))
+    calls = {
+        "conv": (lambda x, w, b: ssm.short_convolution(x, w, b, output_final_state=True), (x, w, b)),
+        "scan": (lambda x, z, A, bc: ssm.selective_scan(x, z, A, bc, bc, z=z, output_final_state=True), (x, z, A, bc)),
+        "norm": (lambda x, z, b: layer_ops.rms_norm_residual(x, z, gate=z, scale=b, post_weight=b, pre_weight=b), (x, z, b)),
+        "norm without weights": (lambda x, z: layer_ops.rms_norm_residual(x, z, scale=0.5)[0], (x, z)),
+    }
+    return {k: (f, [t.to(dev) for t in ts]) for k, (f, ts) in calls.items()}
+
+
+@pytest.mark.parametrize("what", ["conv", "scan", "norm", "norm without weights"])
+def test_a_traced_call_runs_on_its_own_inputs(dev, what):
+    """torch.jit.trace records the operators as calls: the traced function computes on what it is given, not what it was traced with."""
+    f, x = traceable(dev)[what]
+    y = [t.flip(1) if t.dim() == 3 else t for t in x]
+    traced = torch.jit.trace(f, tuple(x), check_trace=False)
+    for inputs in (y, x):
+        got, want = traced(*inputs), f(*inputs)
+        for a, b in zip(got if isinstance(got, tuple) else (got,), want if isinstance(want, tuple) else (want,)):
+            assert torch.equal(a, b)
+
+
+def test_single_tokens_refuse_to_be_traced(dev):
+    from hdla_impl_b200 import ssm
+    x, w, A = torch.ones(2, 8, device=dev), torch.ones(8, 4, device=dev), -torch.ones(8, 4, device=dev)
+    conv, state = torch.zeros(2, 3, 8, device=dev), torch.zeros(2, 8, 4, device=dev)
+    for f in (lambda x: ssm.short_convolution_step(x, conv, w), lambda x: ssm.selective_scan_step(x, x, A, x[:, :4], x[:, :4], state)):
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            torch.jit.trace(f, (x,), check_trace=False)
+    assert float(conv.abs().max()) == 0 and float(state.abs().max()) == 0
