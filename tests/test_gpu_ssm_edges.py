@@ -91,6 +91,46 @@ def test_threads_with_rows_of_different_widths(dev, D):
     assert not wrong, wrong
 
 
+@pytest.mark.parametrize("D", [(4104, 8192), (2056, 4096)])
+def test_threads_with_rows_of_different_widths_at_the_c_entry_points(dev, D):
+    """The same without PyTorch between the calls, so that two threads often stand between a limit and its launch."""
+    import ctypes as C
+    import threading
+    from hdla_impl_b200 import _lib
+    from test_ssm_host import Norm
+    lib = C.CDLL(_lib.lib_path())                            # (prototypes of its own)
+    size = lib.hdla_norm_residual_bwd_workspace_bytes
+    size.restype = C.c_size_t
+    wrong, keep = [], []
+
+    def calls_of(d):
+        x, w, out, f = torch.ones(2, d, device=dev), torch.ones(d, device=dev), torch.empty(8, 2, d, device=dev), torch.empty(2, 2, device=dev)
+        at = lambda k: out[k].data_ptr()  # noqa: E731
+        a = Norm(rows=2, D=d, eps=1e-5, scale_value=1.0, x=x.data_ptr(), post_weight=w.data_ptr(), pre_weight=w.data_ptr(), r=at(0), u=at(1),
+                 factors=f.data_ptr(), dr=x.data_ptr(), du=x.data_ptr(), dx=at(2), dpost_weight=at(3), dpre_weight=at(4))
+        ws = torch.empty(size(C.byref(a)), dtype=torch.uint8, device=dev)
+        keep.extend((x, w, out, f, ws, a))
+        return a, ws
+
+    def work(d, a, ws, stream):
+        for i in range(4000):
+            rc = lib.hdla_norm_residual_fwd(C.byref(a), C.c_void_p(stream)) if i % 2 == 0 else \
+                lib.hdla_norm_residual_bwd(C.byref(a), C.c_void_p(ws.data_ptr()), C.c_size_t(ws.numel()), C.c_void_p(stream))
+            if rc != 0:
+                wrong.append((d, i, rc))
+                return
+
+    streams = [torch.cuda.Stream(dev) for _ in D]
+    threads = [threading.Thread(target=work, args=(d, *calls_of(d), s.cuda_stream)) for d, s in zip(D, streams)]
+    torch.cuda.synchronize()
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not wrong, wrong
+
+
 # --------------------------------------------------------------------------------------------- short convolution
 @pytest.mark.parametrize("xt", [F32, BF])
 @pytest.mark.parametrize("wt,bt", [(BF, F32), (F32, BF), (BF, torch.float16), (BF, torch.float64)])
