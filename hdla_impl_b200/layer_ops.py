@@ -264,6 +264,9 @@ def rms_norm_residual(
     """``v = rms(x) * post_weight``, ``v = v * act(gate)``, ``r = residual + scale * v``, ``u = rms(r) * pre_weight`` with
     ``rms(a) = sqrt(D) a / sqrt(sum(a^2) + eps)``; returns ``(r, u)``, u None without ``pre_weight``.  Each part whose tensor is
     None is left out.  Rows of up to 8192 channels; r has the residual's type, u has x's; u is formed from r before its rounding."""
+    if torch.compiler.is_dynamo_compiling():                  # torch.compile leaves the call out of its graphs
+        return _rms_norm_residual(x, residual, gate=gate, scale=scale, post_weight=post_weight, pre_weight=pre_weight,
+                                  gate_act=gate_act, eps=eps)
     if gate_act not in _GATE_ACTS:
         raise ValueError(f"gate_act {gate_act!r} must be 'sigmoid', 'silu' or None")
     act = _GATE_ACTS[gate_act]
@@ -288,3 +291,6 @@ def rms_norm_residual(
             raise ValueError(f"{name} must be a floating-point vector [D] with D={x.shape[-1]}")
     return _NormResidual.apply(x, residual, gate, scale if torch.is_tensor(scale) else float(scale), post_weight, pre_weight, act,
                                float(eps))
+
+
+_rms_norm_residual = torch.compiler.disable(rms_norm_residual)

@@ -17,7 +17,8 @@ the steps go on with:
 Inputs that are slices of a wider projection (dense along their last dimension) are read where they are.  Under CUDA graph
 capture give ``cu_seqlens`` as an int64 tensor on the GPU; then nothing is copied or waited for, and a replay goes by what the
 tensor then holds.  Rows behind the last offset may hold anything.  The gradients have no graph of their own (no double backward).
-``torch.jit.trace`` records the operators for whole sequences as calls; the steps refuse to be traced.
+``torch.jit.trace`` records the operators for whole sequences as calls; the steps refuse to be traced.  ``torch.compile`` leaves all
+of them out of its graphs.
 """
 from __future__ import annotations
 
@@ -29,6 +30,9 @@ from . import _lib
 from .hrdplr import _plain, autocast_custom_bwd, autocast_custom_fwd
 
 MAX_TAPS, MAX_STATES, MAX_TOKENS = 8, 128, 1 << 30
+# torch.compile leaves the operators out of its graphs: while it looks at one, that one calls itself as torch.compiler.disable
+# gives it.  (As a decorator that would cost a single-token call a tenth of its time.)
+_compiling = torch.compiler.is_dynamo_compiling
 
 
 # ------------------------------------------------------------------------------------------ arguments
@@ -189,6 +193,8 @@ def short_convolution(
     """Depthwise causal convolution: ``y_t = act(bias + sum_{k<W} weight[:, W-1-k] x_{t-k})`` for W of 1 to 8 taps.  The rows
     before a sequence come from ``initial_state`` (its last row the most recent) or are zero; the final state is the last W-1 rows
     of (initial state, x).  Weight and bias may be of other types than x; each is used as it is, in fp32 arithmetic.  With ``cu_seqlens`` B is 1 and n the number of sequences; rows behind the last offset give zeros."""
+    if _compiling():
+        return _short_convolution(x, weight, bias, activation, initial_state, output_final_state, cu_seqlens)
     silu = _silu(activation)
     cu = _offsets(cu_seqlens, x)
     r = (_lib._native or _lib.native()).short_conv(x, weight, bias, silu, initial_state, cu, output_final_state, False)
@@ -207,6 +213,8 @@ def short_convolution_step(
     activation: Optional[str] = "silu",
 ) -> torch.Tensor:
     """One token of each of B sequences through ``short_convolution``; ``state`` (contiguous) moves on by one row in place."""
+    if _compiling():
+        return _short_convolution_step(x, state, weight, bias, activation)
     silu = _silu(activation)
     r = (_lib._native or _lib.native()).short_conv_step(x, state, weight, bias, silu)
     if r is not NotImplemented:
@@ -240,6 +248,8 @@ def selective_scan(
     x, dt, z, B, C are fp32 or bf16, all of one type; A, D, dt_bias and the states are used in fp32, and all arithmetic is fp32.
     The final state is fp32.  Rows of sequences are expected to be finite (an infinite input gives NaN where the formula might
     give an infinity).  With ``cu_seqlens`` B is 1 and n the number of sequences; rows behind the last offset give zeros."""
+    if _compiling():
+        return _selective_scan(x, dt, A, B, C, D, z, dt_bias, dt_softplus, initial_state, output_final_state, cu_seqlens)
     cu = _offsets(cu_seqlens, x)
     softplus = bool(dt_softplus)
     r = (_lib._native or _lib.native()).selective_scan(x, dt, A, B, C, D, z, dt_bias, softplus, initial_state, cu, output_final_state, None)
@@ -263,6 +273,8 @@ def selective_scan_step(
     dt_softplus: bool = True,
 ) -> torch.Tensor:
     """One token of each of B sequences through ``selective_scan``; ``state`` (contiguous, fp32) moves on in place."""
+    if _compiling():
+        return _selective_scan_step(x, dt, A, B, C, state, D, z, dt_bias, dt_softplus)
     softplus = bool(dt_softplus)
     r = (_lib._native or _lib.native()).selective_scan_step(x, dt, A, B, C, D, z, dt_bias, softplus, state)
     if r is not NotImplemented:
@@ -275,3 +287,7 @@ def selective_scan_step(
     if r is NotImplemented:
         raise TypeError("selective_scan_step: unsupported arguments")
     return r
+
+
+_short_convolution, _short_convolution_step, _selective_scan, _selective_scan_step = (
+    torch.compiler.disable(f) for f in (short_convolution, short_convolution_step, selective_scan, selective_scan_step))

@@ -220,3 +220,45 @@ def test_single_tokens_refuse_to_be_traced(dev):
         with pytest.raises(RuntimeError, match="cannot be traced"):
             torch.jit.trace(f, (x,), check_trace=False)
     assert float(conv.abs().max()) == 0 and float(state.abs().max()) == 0
+
+
+@pytest.mark.parametrize("what", ["conv", "scan", "norm", "norm without weights"])
+def test_a_compiled_function_calls_the_operators(dev, what):
+    """torch.compile leaves them out of its graphs: the same bits, gradients among them, and new offsets at every call."""
+    f, x = traceable(dev)[what]
+    torch._dynamo.reset()
+
+    def g(*ts):
+        y = f(*[t * 1 for t in ts])
+        return [t + 0 for t in (y if isinstance(y, tuple) else (y,))]
+
+    def both(h):
+        leaves = [t.detach().requires_grad_(True) for t in x]
+        out = h(*leaves)
+        return [*out, *torch.autograd.grad(out, leaves, [torch.ones_like(o) for o in out])]
+
+    for a, b in zip(both(torch.compile(g, backend="eager")), both(g)):
+        assert torch.equal(a, b)
+
+
+def test_compiled_single_tokens_and_packed_batches(dev):
+    from hdla_impl_b200 import ssm
+    torch._dynamo.reset()
+    g = gen(29)
+    x, w, A, bc = rn(g, 1, 40, 8).to(dev), rn(g, 8, 4).to(dev), -torch.exp(rn(g, 8, 4)).to(dev), rn(g, 1, 40, 4).to(dev)
+
+    def step(x, bc, conv, scan):
+        c = ssm.short_convolution_step(x * 2, conv, w)
+        return ssm.selective_scan_step(c, x, A, bc, bc, scan) + 1
+
+    def packed(x, bc, cu):
+        c, _ = ssm.short_convolution(x * 2, w, cu_seqlens=cu)
+        return ssm.selective_scan(c, x, A, bc, bc, cu_seqlens=cu)[0] + 1
+
+    fast = torch.compile(step, backend="eager"), torch.compile(packed, backend="eager")
+    states = [[torch.zeros(1, 3, 8, device=dev), torch.zeros(1, 8, 4, device=dev)] for _ in range(2)]
+    for t in range(4):
+        assert torch.equal(fast[0](x[:, t], bc[:, t], *states[0]), step(x[:, t], bc[:, t], *states[1]))
+    assert all(torch.equal(a, b) for a, b in zip(*states))
+    for cut in range(3, 15):
+        assert torch.equal(fast[1](x, bc, [0, cut, 40]), packed(x, bc, [0, cut, 40]))
