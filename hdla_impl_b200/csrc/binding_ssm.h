@@ -301,16 +301,16 @@ ScanGrads scan_backward(const ScanIn& i, const Tensor& ckpt, const Tensor& dy_, 
 }
 
 struct ScanNode : torch::autograd::Node {
-    Saved x, dt, A, B, C, D, z, bias, h0, cu;
-    Tensor ckpt;                                     // read only: a second backward finds it as it was
+    // ckpt: forward's states, the largest of these by far, so that hooks (offloading, activation checkpointing) get it too; read
+    // only, a second backward finds it as it was
+    Saved x, dt, A, B, C, D, z, bias, h0, cu, ckpt;
     bool softplus = false;
     at::ScalarType A_type, D_type, bias_type, h0_type;
     std::vector<int64_t> B_size, C_size;
     std::string name() const override { return "HdlaSelectiveScanBackward"; }
     void release_variables() override {
         std::lock_guard<std::mutex> lock(mutex_);
-        for (Saved* s : {&x, &dt, &A, &B, &C, &D, &z, &bias, &h0, &cu}) s->var.reset_data();
-        ckpt = Tensor();
+        for (Saved* s : {&x, &dt, &A, &B, &C, &D, &z, &bias, &h0, &cu, &ckpt}) s->var.reset_data();
     }
     variable_list apply(variable_list&& grads) override {
         std::lock_guard<std::mutex> lock(mutex_);
@@ -320,7 +320,7 @@ struct ScanNode : torch::autograd::Node {
         const char* me = "HdlaSelectiveScanBackward";
         const ScanIn i{unpack_saved(x, me), unpack_saved(dt, me), A.get(me), grouped(unpack_saved(B, me)), grouped(unpack_saved(C, me)),
                        D.get(me), unpack_saved(z, me), bias.get(me), h0.get(me), cu.get(me), softplus};
-        ScanGrads g = scan_backward(i, ckpt, grads[0], dht);
+        ScanGrads g = scan_backward(i, ckpt.get(me), grads[0], dht);
         return {g.dx, g.ddt, as_type(g.dA, A_type), g.dB.view(B_size), g.dC.view(C_size), as_type(g.dD, D_type), g.dz,
                 as_type(g.dbias, bias_type), as_type(g.dh0, h0_type)};
     }
@@ -346,7 +346,7 @@ std::pair<Tensor, Tensor> scan_op(const ScanCall& c, bool want_ht) {
             node->x.save(i.x); node->dt.save(i.dt); node->A.save(i.A); node->D.save(i.D); node->z.save(i.z);
             node->B.save(*c.B); node->C.save(*c.C);
             node->bias.save(i.bias); node->h0.save(i.h0); node->cu.save(i.cu);
-            node->ckpt = r.ckpt;
+            node->ckpt.save(r.ckpt);
             node->softplus = c.softplus;
             auto type = [](const Tensor& t) { return t.defined() ? t.scalar_type() : at::kFloat; };
             node->A_type = type(*c.A); node->D_type = type(*c.D); node->bias_type = type(*c.bias); node->h0_type = type(*c.h0);
@@ -522,15 +522,13 @@ NormIn norm_in(const NormCall& c) {
 }
 
 struct NormResidualNode : torch::autograd::Node {
-    Saved x, r, g, post, pre, scale;
-    Tensor factors;                                  // read only
+    Saved x, r, g, post, pre, scale, factors;
     NormIn rest;                                     // the numbers; no tensors
     at::ScalarType post_type = at::kFloat, pre_type = at::kFloat, scale_type = at::kFloat;
     std::string name() const override { return "HdlaNormResidualBackward"; }
     void release_variables() override {
         std::lock_guard<std::mutex> lock(mutex_);
-        for (Saved* s : {&x, &r, &g, &post, &pre, &scale}) s->var.reset_data();
-        factors = Tensor();
+        for (Saved* s : {&x, &r, &g, &post, &pre, &scale, &factors}) s->var.reset_data();
     }
     variable_list apply(variable_list&& grads) override {
         std::lock_guard<std::mutex> lock(mutex_);
@@ -540,7 +538,7 @@ struct NormResidualNode : torch::autograd::Node {
         const char* me = "HdlaNormResidualBackward";
         NormIn i = rest;
         i.x = x.get(me); i.r = r.get(me); i.g = g.get(me); i.post = post.get(me); i.pre = pre.get(me); i.scale = scale.get(me);
-        NormGrads d = norm_backward(i, factors, grads[0], du);
+        NormGrads d = norm_backward(i, factors.get(me), grads[0], du);
         return {d.dx, d.dr, d.dg, as_type(d.dscale, scale_type), as_type(d.dpost, post_type), as_type(d.dpre, pre_type)};
     }
 };
@@ -557,7 +555,7 @@ std::pair<Tensor, Tensor> norm_residual_op(const NormCall& c) {
         if (grad) {
             node = make_node<NormResidualNode>();
             node->x.save(i.x); node->r.save(i.r); node->g.save(i.g); node->post.save(i.post); node->pre.save(i.pre); node->scale.save(i.scale);
-            node->factors = out.factors;
+            node->factors.save(out.factors);
             node->rest.scale_value = i.scale_value; node->rest.eps = i.eps; node->rest.act = i.act; node->rest.w_type = i.w_type;
             if (c.post->defined()) node->post_type = c.post->scalar_type();
             if (c.pre->defined()) node->pre_type = c.pre->scalar_type();

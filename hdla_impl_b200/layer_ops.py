@@ -226,12 +226,12 @@ class _NormResidual(torch.autograd.Function):
     def forward(ctx, x, residual, gate, scale, post_weight, pre_weight, act, eps):
         ctx.scale = None if torch.is_tensor(scale) else scale
         ctx.act, ctx.eps = act, eps
-        ctx.save_for_backward(x, residual, gate, scale if ctx.scale is None else None, post_weight, pre_weight)
         keep = any(torch.is_tensor(t) and t.requires_grad for t in (x, residual, gate, scale, post_weight, pre_weight))
         out = _lib.native().norm_residual(*_NormResidual._args(ctx, (x, residual, gate, scale, post_weight, pre_weight)), keep)
         if out is NotImplemented:
             raise TypeError("rms_norm_residual: unsupported arguments")
-        r, u, ctx.factors = out
+        r, u, factors = out
+        ctx.save_for_backward(x, residual, gate, scale if ctx.scale is None else None, post_weight, pre_weight, factors)
         return r, u
 
     @staticmethod
@@ -242,8 +242,8 @@ class _NormResidual(torch.autograd.Function):
     @staticmethod
     @_op.autocast_custom_bwd
     def backward(ctx, dr, du):
-        g = _lib.native().norm_residual_backward(*_NormResidual._args(ctx, ctx.saved_tensors), ctx.factors,
-                                                 _op._plain(dr), _op._plain(du))
+        *tensors, factors = ctx.saved_tensors
+        g = _lib.native().norm_residual_backward(*_NormResidual._args(ctx, tensors), _op._plain(factors), _op._plain(dr), _op._plain(du))
         return (*g, None, None)
 
 

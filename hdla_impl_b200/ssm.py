@@ -157,17 +157,16 @@ class _SelectiveScan(torch.autograd.Function):
                                          want, keep)
         if r is NotImplemented:
             raise TypeError("selective_scan: unsupported arguments")
-        y, ht, ctx.checkpoints = r
+        y, ht, checkpoints = r
         ctx.softplus = softplus
-        ctx.save_for_backward(x, dt, A, B, C, D, z, dt_bias, h0, cu)
+        ctx.save_for_backward(x, dt, A, B, C, D, z, dt_bias, h0, cu, checkpoints)
         return y, ht
 
     @staticmethod
     @autocast_custom_bwd
     def backward(ctx, dy, dht):
-        x, dt, A, B, C, D, z, dt_bias, h0, cu = [_plain(t) for t in ctx.saved_tensors]
-        g = _lib.native().selective_scan_backward(x, dt, A, B, C, D, z, dt_bias, ctx.softplus, h0, cu, ctx.checkpoints, _plain(dy),
-                                                  _plain(dht))
+        x, dt, A, B, C, D, z, dt_bias, h0, cu, checkpoints = [_plain(t) for t in ctx.saved_tensors]
+        g = _lib.native().selective_scan_backward(x, dt, A, B, C, D, z, dt_bias, ctx.softplus, h0, cu, checkpoints, _plain(dy), _plain(dht))
         return (*g[:8], None, g[8], None, None)
 
 

@@ -262,3 +262,64 @@ def test_compiled_single_tokens_and_packed_batches(dev):
     assert all(torch.equal(a, b) for a, b in zip(*states))
     for cut in range(3, 15):
         assert torch.equal(fast[1](x, bc, [0, cut, 40]), packed(x, bc, [0, cut, 40]))
+
+
+# --------------------------------------------------------------------------------------------- what is kept for backward
+def scan_for_memory(dev):
+    """A scan whose checkpoints (8 bytes a token and channel) outweigh all else: (function, leaves, gradient of y, bytes of y, of them)."""
+    from hdla_impl_b200 import ssm
+    g = torch.Generator(device=dev).manual_seed(3)
+    B, T, D, N = 2, 1024, 512, 16
+    rnd = lambda *s: torch.randn(*s, generator=g, device=dev)  # noqa: E731
+    t = [rnd(B, T, D), rnd(B, T, D), -torch.exp(rnd(D, N)), rnd(B, T, N), rnd(B, T, N)]
+    for v in t:
+        v.requires_grad_(True)
+    return (lambda *t: ssm.selective_scan(*t)[0]), t, rnd(B, T, D), B * T * D * 4, B * T // 8 * D * N * 4
+
+
+def kept(f):
+    """(what f returns, the bytes that it has left allocated)"""
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    y = f()
+    torch.cuda.synchronize()
+    return y, torch.cuda.memory_allocated() - before
+
+
+@pytest.mark.parametrize("how", ["checkpoint", "save_on_cpu", "subclass on cpu"])
+def test_the_scans_checkpoints_go_through_saved_tensor_hooks(dev, how):
+    """Activation checkpointing and offloading leave nothing of them on the GPU until backward, and the gradients are the same bits."""
+    from torch.utils.checkpoint import checkpoint
+
+    class Mine(torch.Tensor):
+        pass
+
+    f, t, dy, size, saved = scan_for_memory(dev)
+    y, bytes_ = kept(lambda: f(*t))
+    assert bytes_ >= size + saved
+    want = torch.autograd.grad(y, t, dy)
+
+    def call():
+        if how == "checkpoint":
+            return checkpoint(f, *t, use_reentrant=False)
+        with torch.autograd.graph.save_on_cpu():
+            return f(*t) if how == "save_on_cpu" else f(t[0].as_subclass(Mine), *t[1:])
+
+    y2, bytes_ = kept(call)
+    assert bytes_ < size + saved // 4
+    assert torch.equal(y2.as_subclass(torch.Tensor), y)
+    for a, b in zip(torch.autograd.grad(y2, t, dy), want):
+        assert torch.equal(a.as_subclass(torch.Tensor), b)
+
+
+def test_the_norms_factors_go_through_saved_tensor_hooks(dev):
+    from hdla_impl_b200 import layer_ops
+    g = gen(5)
+    x, w, do = rn(g, 40, 64).to(dev).requires_grad_(True), rn(g, 64).to(dev).requires_grad_(True), rn(g, 40, 64).to(dev)
+    seen = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: seen.append(tuple(t.shape)) or t.cpu(), lambda t: t.to(dev)):
+        r, u = layer_ops.rms_norm_residual(x, post_weight=w, pre_weight=w)
+    r2, u2 = layer_ops.rms_norm_residual(x, post_weight=w, pre_weight=w)
+    assert (40, 2) in seen
+    for a, b in zip(torch.autograd.grad([r, u], [x, w], [do, do]), torch.autograd.grad([r2, u2], [x, w], [do, do])):
+        assert torch.equal(a, b)
