@@ -283,8 +283,10 @@ ScanOut scan_forward(const ScanIn& i, bool want_ht, bool keep) {
     return r;
 }
 struct ScanGrads { Tensor dx, ddt, dA, dB, dC, dD, dz, dbias, dh0; };
-ScanGrads scan_backward(const ScanIn& i, const Tensor& ckpt, const Tensor& dy_, const Tensor& dht_) {
+// (without the forward pass's checkpoints it runs once more)
+ScanGrads scan_backward(const ScanIn& i, Tensor ckpt, const Tensor& dy_, const Tensor& dht_) {
     c10::cuda::CUDAGuard guard(i.x.device());
+    if (!ckpt.defined()) ckpt = scan_forward(i, false, true).ckpt;
     HdlaScanArgs a = scan_args(i);
     const auto st = i.x.scalar_type();
     const Tensor dy = grad_in(dy_, st), dht = grad_in(dht_, at::kFloat);
@@ -340,7 +342,7 @@ std::pair<Tensor, Tensor> scan_op(const ScanCall& c, bool want_ht) {
         at::NoGradGuard no_grad;
         c10::cuda::CUDAGuard guard(c.x->device());
         const ScanIn i = scan_in(c);
-        r = scan_forward(i, want_ht, grad);
+        r = scan_forward(i, want_ht, grad && !env_is_1("HDLA_RECOMPUTE"));
         if (grad) {
             node = make_node<ScanNode>();
             node->x.save(i.x); node->dt.save(i.dt); node->A.save(i.A); node->D.save(i.D); node->z.save(i.z);
@@ -410,11 +412,11 @@ PyObject* py_selective_scan(PyObject*, PyObject* const* av, Py_ssize_t n) {
         return nullptr;
     return bare ? tuple_of({&r.y, &r.ht, &r.ckpt}) : tuple_of({&r.y, &r.ht});
 }
-// selective_scan_backward(..., checkpoints, dy or None, dht or None) -> gradients of (x, dt, A, B, C, D, z, dt_bias, h0)
+// selective_scan_backward(..., checkpoints or None, dy or None, dht or None) -> gradients of (x, dt, A, B, C, D, z, dt_bias, h0)
 PyObject* py_selective_scan_backward(PyObject*, PyObject* const* av, Py_ssize_t n) {
     if (n != 14) { PyErr_SetString(PyExc_TypeError, "selective_scan_backward takes 14 arguments"); return nullptr; }
     ScanCall c;
-    const Tensor *ck = arg(av[11]), *dy = arg(av[12], true), *dht = arg(av[13], true);
+    const Tensor *ck = arg(av[11], true), *dy = arg(av[12], true), *dht = arg(av[13], true);
     if (!scan_call(av, 2, c) || !ck || !dy || !dht) {
         PyErr_SetString(PyExc_TypeError, "selective_scan_backward: arguments of another kind than the forward call's");
         return nullptr;
@@ -424,7 +426,7 @@ PyObject* py_selective_scan_backward(PyObject*, PyObject* const* av, Py_ssize_t 
             at::NoGradGuard no_grad;
             const ScanIn i = scan_in(c);
             const HdlaScanArgs a = scan_args(i);
-            if (ck->scalar_type() != at::kFloat || !ck->is_contiguous() || ck->numel() * sizeof(float) < ssm.scan_checkpoint_bytes(&a))
+            if (ck->defined() && (ck->scalar_type() != at::kFloat || !ck->is_contiguous() || ck->numel() * sizeof(float) < ssm.scan_checkpoint_bytes(&a)))
                 throw std::runtime_error("selective_scan_backward: these are not the forward call's checkpoints");
             g = scan_backward(i, *ck, *dy, *dht);
             g.dB = g.dB.view(c.B->sizes()); g.dC = g.dC.view(c.C->sizes());

@@ -27,7 +27,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .hrdplr import _plain, autocast_custom_bwd, autocast_custom_fwd
+from .hrdplr import _plain, autocast_custom_bwd, autocast_custom_fwd, save_workspace_default
 
 MAX_TAPS, MAX_STATES, MAX_TOKENS = 8, 128, 1 << 30
 # torch.compile leaves the operators out of its graphs: while it looks at one, that one calls itself as torch.compiler.disable
@@ -152,7 +152,8 @@ class _SelectiveScan(torch.autograd.Function):
     @staticmethod
     @autocast_custom_fwd
     def forward(ctx, x, dt, A, B, C, D, z, dt_bias, softplus, h0, cu, want):
-        keep = any(isinstance(t, torch.Tensor) and t.requires_grad for t in (x, dt, A, B, C, D, z, dt_bias, h0))
+        keep = save_workspace_default() and any(
+            isinstance(t, torch.Tensor) and t.requires_grad for t in (x, dt, A, B, C, D, z, dt_bias, h0))
         r = _lib.native().selective_scan(*[_plain(t) for t in (x, dt, A, B, C, D, z, dt_bias)], softplus, _plain(h0), _plain(cu),
                                          want, keep)
         if r is NotImplemented:
@@ -245,7 +246,9 @@ def selective_scan(
     """Selective scan over D channels of N states (1 to 128), groups of D / G channels sharing B and C:
     ``d_t = softplus(dt_t + dt_bias)``, ``h_t = exp(d_t A) h_{t-1} + d_t x_t B_t``, ``y_t = (C_t . h_t + D x_t) silu(z_t)``.
     x, dt, z, B, C are fp32 or bf16, all of one type; A, D, dt_bias and the states are used in fp32, and all arithmetic is fp32.
-    The final state is fp32.  Rows of sequences are expected to be finite (an infinite input gives NaN where the formula might
+    The final state is fp32.  A call that needs gradients keeps its states at every eighth token for backward, in fp32: N / 2 bytes a
+    token and channel (N rounded up to 8, 16, 32, 64 or 128; at 16 states four times x in bf16).  With HDLA_RECOMPUTE=1 in the
+    environment nothing of them is kept, and backward runs the forward pass once more.  Rows of sequences are expected to be finite (an infinite input gives NaN where the formula might
     give an infinity).  With ``cu_seqlens`` B is 1 and n the number of sequences; rows behind the last offset give zeros."""
     if _compiling():
         return _selective_scan(x, dt, A, B, C, D, z, dt_bias, dt_softplus, initial_state, output_final_state, cu_seqlens)

@@ -312,6 +312,22 @@ def test_the_scans_checkpoints_go_through_saved_tensor_hooks(dev, how):
         assert torch.equal(a.as_subclass(torch.Tensor), b)
 
 
+@pytest.mark.parametrize("subclass", [False, True])
+def test_the_scans_checkpoints_can_be_done_without(dev, monkeypatch, subclass):
+    """HDLA_RECOMPUTE=1, as for the chunked operator: nothing of them is kept, and the gradients are the same bits, twice."""
+    class Mine(torch.Tensor):
+        pass
+
+    f, t, dy, size, saved = scan_for_memory(dev)
+    want = torch.autograd.grad(f(*t), t, dy)
+    monkeypatch.setenv("HDLA_RECOMPUTE", "1")
+    y, bytes_ = kept(lambda: f(t[0].as_subclass(Mine) if subclass else t[0], *t[1:]))
+    assert bytes_ < size + saved // 4
+    for again in (True, False):
+        for a, b in zip(torch.autograd.grad(y, t, dy, retain_graph=again), want):
+            assert torch.equal(a.as_subclass(torch.Tensor), b)
+
+
 def test_the_norms_factors_go_through_saved_tensor_hooks(dev):
     from hdla_impl_b200 import layer_ops
     g = gen(5)
