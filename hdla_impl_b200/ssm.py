@@ -22,6 +22,7 @@ of them out of its graphs.
 """
 from __future__ import annotations
 
+import operator
 from typing import Optional, Tuple
 
 import torch
@@ -47,7 +48,11 @@ def _offsets(cu_seqlens, x) -> Optional[torch.Tensor]:
         if cu_seqlens.is_floating_point() or cu_seqlens.dim() != 1:
             raise ValueError("cu_seqlens must be a vector of integers")
         return cu_seqlens.to(torch.int64).contiguous()
-    host = cu_seqlens.tolist() if isinstance(cu_seqlens, torch.Tensor) else [int(c) for c in cu_seqlens]
+    try:
+        host = [operator.index(c) for c in (cu_seqlens.tolist() if isinstance(cu_seqlens, torch.Tensor) else cu_seqlens)]
+    except TypeError:
+        raise ValueError("cu_seqlens must be a vector of integers") from None
+    _need(x.dim() == 3, f"x must have 3 dimensions [B, T, D], got {x.dim()}")
     T = x.shape[1]
     if len(host) < 2 or host[0] != 0 or host[-1] > T or any(b < a for a, b in zip(host, host[1:])):
         raise ValueError(f"cu_seqlens {host} must rise from 0 to at most T={T}")
