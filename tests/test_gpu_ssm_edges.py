@@ -339,3 +339,126 @@ def test_the_norms_factors_go_through_saved_tensor_hooks(dev):
     assert (40, 2) in seen
     for a, b in zip(torch.autograd.grad([r, u], [x, w], [do, do]), torch.autograd.grad([r2, u2], [x, w], [do, do])):
         assert torch.equal(a, b)
+
+
+# --------------------------------------------------------------------------------------------- offsets
+@pytest.mark.parametrize("given,taken", [([0, -3, 20, 50], [0, 0, 20, 50]), ([5, 20, 50, 50], [0, 20, 50, 50]), ([0, 20, 1000, 1 << 40], [0, 20, 50, 50]),
+                                         ([-(1 << 40), -7, 0, 33], [0, 0, 0, 33])])
+def test_offsets_on_the_gpu_are_cut_to_the_batch(dev, given, taken):
+    """Offsets on the GPU are not looked at by the host: the first counts as 0, those outside 0..T are cut to that range.  Outputs,
+    states and all gradients are those of the offsets that result."""
+    from hdla_impl_b200 import ssm
+    g = gen(50)
+    T, D, N = 50, 16, 4
+    t = {"x": rn(g, 1, T, D), "w": rn(g, D, 4), "h": rn(g, 3, 3, D), "dt": rn(g, 1, T, D), "A": -torch.exp(rn(g, D, N)), "B": rn(g, 1, T, N),
+         "C": rn(g, 1, T, N), "z": rn(g, 1, T, D), "s": rn(g, 3, D, N)}
+    dy, dh, ds = rn(g, 1, T, D).to(dev), rn(g, 3, 3, D).to(dev), rn(g, 3, D, N).to(dev)
+
+    def f(cu):
+        v = {k: a.to(dev).requires_grad_(True) for k, a in t.items()}
+        c, h = ssm.short_convolution(v["x"], v["w"], initial_state=v["h"], output_final_state=True, cu_seqlens=cu)
+        y, s = ssm.selective_scan(v["x"], v["dt"], v["A"], v["B"], v["C"], z=v["z"], initial_state=v["s"], output_final_state=True, cu_seqlens=cu)
+        return [c, h, y, s, *torch.autograd.grad([c, h, y, s], list(v.values()), [dy, dh, dy, ds])]
+
+    for a, b in zip(f(torch.tensor(given, device=dev)), f(torch.tensor(taken, device=dev))):
+        assert bool(torch.isfinite(a).all()) and torch.equal(a, b)
+
+
+# --------------------------------------------------------------------------------------------- gradients that are long sums
+# Inputs without signs, so that no sum cancels and a lost or doubled token shows in every entry: errors are taken entry by entry,
+# relative to the sum of the magnitudes of what it consists of.  u = 2^-24 is a rounding of fp32.
+U = 2.0 ** -24
+
+
+def entries_close(got, ref, size, tol, name):
+    assert got.dtype == F32 and got.shape == ref.shape
+    e = float(((got.cpu().double() - ref).abs() / size).max())
+    assert e <= tol, f"{name}: {e:.3g} > {tol:.3g}"
+
+
+def scan64(x, dt, dt2, A, B, C, D, z, bias, bias2, h0, cu):
+    """The definition, with the time steps of the decays (dt2, bias2) apart from those of the inputs: their gradients have opposite signs."""
+    T = x.shape[1]
+    sp = lambda v: torch.clamp(v, min=0) + torch.log1p(torch.exp(-v.abs()))  # noqa: E731
+    d, d2 = sp(dt + bias), sp(dt2 + bias2)
+    per = x.shape[2] // B.shape[2]
+    ys, first, h = [], dict(zip(cu, range(len(cu) - 1))), None
+    for t in range(T):
+        if t in first:
+            h = h0[first[t]][None]
+        h = torch.exp(d2[:, t, :, None] * A) * h + (d[:, t] * x[:, t])[..., None] * B[:, t].repeat_interleave(per, 1)
+        ys.append(((C[:, t].repeat_interleave(per, 1) * h).sum(-1) + D * x[:, t]) * z[:, t] / (1 + torch.exp(-z[:, t])))
+    return torch.stack(ys, 1)
+
+
+@pytest.mark.parametrize("T,D,N,G,dtype,slow,cu", [(1300, 8, 16, 1, F32, 64, None), (1300, 8, 16, 2, BF, 64, [0, 1, 640, 1300]), (200, 24, 5, 1, F32, 1e6, None),
+                                                   (700, 8, 128, 2, BF, 64, None), (900, 12, 8, 1, F32, 16, [0, 899, 900])])
+def test_every_token_is_in_the_weights_gradients_once(dev, T, D, N, G, dtype, slow, cu):
+    """Decays of 1 / slow a token and more: a state remembers min(T, slow) tokens.  Each of them costs a rounding, the exponential's
+    4 u and what the rounding of its argument does, 5 u in all, for the state and for its gradient; 10 u each for the time step in
+    the exponent; T u at most for a sum of T terms without signs; 64 u for the rest.  A token is 1 / T of such a sum."""
+    from hdla_impl_b200 import ssm
+    g = gen(T)
+    pos = lambda *s, dtype=dtype: (0.5 + torch.rand(*s, generator=g)).to(dtype)  # noqa: E731
+    seqs = [0, T] if cu is None else cu
+    v = {"x": pos(1, T, D), "dt": torch.randn(1, T, D, generator=g).to(dtype), "A": -(1 + torch.rand(D, N, generator=g)) / slow * 4, "B": pos(1, T, G, N),
+         "C": pos(1, T, G, N), "D": pos(D, dtype=F32), "z": pos(1, T, D), "bias": 0.5 + torch.rand(D, generator=g), "h0": pos(len(seqs) - 1, D, N, dtype=F32)}
+    dy = pos(1, T, D)
+    own = {k: a.to(dev).requires_grad_(k in ("A", "D", "bias", "h0")) for k, a in v.items()}
+    y, _ = ssm.selective_scan(own["x"], own["dt"], own["A"], own["B"], own["C"], D=own["D"], z=own["z"], dt_bias=own["bias"], initial_state=own["h0"],
+                              cu_seqlens=cu)
+    names = ["A", "D", "bias", "h0"]
+    got = dict(zip(names, torch.autograd.grad(y, [own[k] for k in names], dy.to(dev))))
+    ref = {k: a.double().requires_grad_(k in names) for k, a in v.items()}
+    bias2 = ref["bias"].detach().clone().requires_grad_(True)
+    r = scan64(ref["x"], ref["dt"], ref["dt"], ref["A"], ref["B"], ref["C"], ref["D"], ref["z"], ref["bias"], bias2, ref["h0"], seqs)
+    want = dict(zip([*names, "bias2"], torch.autograd.grad(r, [*(ref[k] for k in names), bias2], dy.double())))
+    size = {k: w.abs() for k, w in want.items()}
+    size["bias"] = size["bias"] + size["bias2"]
+    want["bias"] = want["bias"] + want["bias2"]
+    tol = (2 * (10 + 5 * min(T, slow)) + T + 64) * U
+    assert tol < 0.5 / T
+    for k in names:
+        entries_close(got[k], want[k], size[k], tol, "d" + k)
+
+
+@pytest.mark.parametrize("rows,D,dtype,rt", [(1300, 256, BF, BF), (1300, 256, BF, F32), (3001, 1001, F32, F32), (700, 2048, BF, F32), (900, 5000, BF, F32)])
+def test_every_row_is_in_the_norms_weights_gradients_once(dev, rows, D, dtype, rt):
+    """A factor of a row costs the roundings of a tree over D squares, 32 u, and its root's 4 u; the gate 16 u; a block's rows and
+    the blocks one after another, at most rows / 100 + 64 u."""
+    from hdla_impl_b200 import layer_ops
+    g = gen(D)
+    pos = lambda *s, dtype=dtype: (0.5 + torch.rand(*s, generator=g)).to(dtype)  # noqa: E731
+    x, r, gate, do = pos(rows, D), pos(rows, D, dtype=rt), pos(rows, D), pos(rows, D)
+    w = {k: pos(D, dtype=F32) for k in ("scale", "post_weight", "pre_weight")}
+    tol = (32 + 4 + 16 + 64 + 64 + rows / 100) * U
+    assert tol < 0.5 / rows
+    # the scale's and the first norm's gradients where there is no second norm, whose own gradient is a difference
+    for names in (("scale", "post_weight"), ("pre_weight", "scale", "post_weight")):
+        own = {k: w[k].to(dev).requires_grad_(True) for k in names}
+        out = layer_ops.rms_norm_residual(x.to(dev), r.to(dev), gate=gate.to(dev), **own)
+        last, up = (out[0], do.to(rt)) if len(names) == 2 else (out[1], do)
+        ref = {k: w[k].double().requires_grad_(True) for k in names}
+        ro = orc.norm_residual(x.double(), r.double(), gate.double(), ref["scale"], ref["post_weight"], ref.get("pre_weight"))
+        want = torch.autograd.grad(ro[0] if len(names) == 2 else ro[1], list(ref.values()), up.double())
+        got = torch.autograd.grad(last, list(own.values()), up.to(dev))
+        for k, a, b in list(zip(names, got, want))[:1 if len(names) == 3 else 2]:
+            entries_close(a, b, b.abs(), tol, "d" + k)
+
+
+@pytest.mark.parametrize("B,T,D,W,dtype,cu", [(2, 3001, 40, 4, BF, None), (1, 5000, 33, 7, F32, [0, 1, 2, 2400, 5000]), (3, 129, 64, 2, F32, None)])
+def test_every_token_is_in_the_convolutions_weights_gradients_once(dev, B, T, D, W, dtype, cu):
+    """W + 1 roundings and a sigmoid's 16 u a token; a strip of 128 tokens, eight strips and the blocks' sums one after another."""
+    from hdla_impl_b200 import ssm
+    g = gen(W)
+    pos = lambda *s, dtype=dtype: (0.5 + torch.rand(*s, generator=g)).to(dtype)  # noqa: E731
+    n = B if cu is None else len(cu) - 1
+    x, w, b, h0, dy = pos(B, T, D), pos(D, W, dtype=F32), pos(D, dtype=F32), pos(n, W - 1, D), pos(B, T, D)
+    own = [w.to(dev).requires_grad_(True), b.to(dev).requires_grad_(True)]
+    got = torch.autograd.grad(ssm.short_convolution(x.to(dev), *own, initial_state=h0.to(dev), cu_seqlens=cu)[0], own, dy.to(dev))
+    ref = [w.double().requires_grad_(True), b.double().requires_grad_(True)]
+    want = torch.autograd.grad(orc.short_conv(x.double(), *ref, "silu", h0.double(), cu)[0], ref, dy.double())
+    tol = (16 + W + 1 + 128 + 8 + 32 + B * T / 1024) * U
+    assert tol < 0.5 / (B * T)
+    for k, a, q in zip("wb", got, want):
+        entries_close(a, q, q.abs(), tol, "d" + k)
