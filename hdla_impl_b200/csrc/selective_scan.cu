@@ -1,9 +1,10 @@
 // Selective state space scan, forward and single tokens (the layout of the work is in selective_scan.cuh).
 //
-// What bounds the forward pass: the exponentials, one per (token, channel, state) and four more per (token, channel), 16 a clock
-// and SM (62 % of their peak with two channels a lane), with shared-memory cycles (59 %) and issue slots (52 %) close behind;
-// HBM traffic takes a third of that at N = 16.  (A quarter of the exponentials as polynomials on the multiply-add pipes made
-// it slower: 835 -> 879 us.)  8 x 4096 x 2048, N = 16, bf16, with checkpoints: 575 us.
+// What the forward pass cannot do without: the exponentials, one per (token, channel, state) and four more per (token, channel), 16
+// a clock and SM; HBM traffic takes a third of that at N = 16.  8 x 4096 x 2048, N = 16, bf16, with checkpoints: 578 us, 1.9 times
+// its exponentials; where rows are cut the maps take them a second time (one row of 65536 tokens: 2.3 times).  No pipe is full
+// (with two channels a lane the exponentials' 62 %, shared-memory cycles 59 %, issue slots 52 %): the phases of a tile between its
+// barriers do not overlap.  (A quarter of the exponentials as polynomials on the multiply-add pipes made it slower: 835 -> 879 us.)
 #include "selective_scan.cuh"
 
 namespace hdla {
@@ -305,7 +306,8 @@ int scan_lanes(int N) {
     return nl;
 }
 
-// Channels a lane, and segments.  Five blocks an SM are resident forward, three backward, and about so many hide the latencies.
+// Channels a lane, and segments.  Resident on an SM are four blocks forward with one channel a lane, five with two (and of the maps),
+// three backward, and about so many hide the latencies.
 // Two channels a lane are cheaper in shared-memory cycles than one, one channel a lane gives twice the blocks.  Cutting rows
 // runs the recurrence once more for the maps, and pays only where too few blocks would be left.  Measured at N = 16, 8 rows of
 // 2048 channels, T = 4096.  Forward: one channel, whole rows (512 blocks) 573 us; two channels, whole rows (256 blocks) 729 us;
@@ -337,7 +339,8 @@ ScanPlan scan_plan(const HdlaScanArgs& a, bool backward) {
     return r;
 }
 // Tiles of channels that keep shares of dB and dC of their own: all, unless those shares would take over 1 GiB (many states
-// make narrow tiles).  Then the tiles take turns, a launch after another, and add to the shares of those before them.
+// make narrow tiles); then as many as 1 GiB holds, one at least.  The tiles take turns, a launch after another, and add to the
+// shares of those before them.
 int scan_slots(const HdlaScanArgs& a, const ScanPlan& r) {
     const size_t each = (size_t)a.B * a.T * a.G * 8 * scan_lanes(a.N) * sizeof(float), most = (size_t(1) << 30) / each;
     return most >= (size_t)r.tiles ? r.tiles : most < 1 ? 1 : (int)most;

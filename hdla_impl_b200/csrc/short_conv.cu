@@ -6,7 +6,8 @@
 // has just brought to L2.  Several tokens are requested at a time, and forward the next ones before these are worked on.  Four
 // channels a thread and not eight (16 bytes of bf16): the taps, their sums and the histories are what fills the registers, and
 // with half of them twice the warps hide the latency (forward 100 -> 61 us, backward 262 -> 148 us at 32768 x 2048, W = 4).
-// There forward now takes 55 us = 4.9 TB/s (0.76 of the measured copy), backward 104 us = 3.9 TB/s (0.60) and its sums 10 us.
+// There forward now takes 55 us = 4.9 TB/s (0.76 of the measured copy), backward 106 us = 3.8 TB/s (0.59) and its sums 10 us;
+// 16384 x 2048 in fp32: 49 us = 5.5 TB/s (0.85) and 101 us = 4.0 TB/s (0.62).
 #include "ssm.cuh"
 
 namespace hdla {

@@ -263,7 +263,8 @@ def rms_norm_residual(
 ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """``v = rms(x) * post_weight``, ``v = v * act(gate)``, ``r = residual + scale * v``, ``u = rms(r) * pre_weight`` with
     ``rms(a) = sqrt(D) a / sqrt(sum(a^2) + eps)``; returns ``(r, u)``, u None without ``pre_weight``.  Each part whose tensor is
-    None is left out.  Rows of up to 8192 channels; r has the residual's type, u has x's; u is formed from r before its rounding."""
+    None is left out.  eps stands beside the sum of a row's squares: for weights of a norm with ``mean(a^2) + e`` give ``eps=e * D``.
+    Rows of up to 8192 channels; r has the residual's type, u has x's; u is formed from r before its rounding."""
     if torch.compiler.is_dynamo_compiling():                  # torch.compile leaves the call out of its graphs
         return _rms_norm_residual(x, residual, gate=gate, scale=scale, post_weight=post_weight, pre_weight=pre_weight,
                                   gate_act=gate_act, eps=eps)

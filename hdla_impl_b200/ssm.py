@@ -16,7 +16,9 @@ the steps go on with:
 
 Inputs that are slices of a wider projection (dense along their last dimension) are read where they are.  Under CUDA graph
 capture give ``cu_seqlens`` as an int64 tensor on the GPU; then nothing is copied or waited for, and a replay goes by what the
-tensor then holds.  Rows behind the last offset may hold anything.  The gradients have no graph of their own (no double backward).
+tensor then holds.  Offsets on the host are checked; those on the GPU are not looked at before the kernels, which take the first one
+as 0 and cut the others to 0..T: they must not fall (nothing outside the tensors is touched if they do, but what comes out means
+nothing).  Rows behind the last offset may hold anything.  The gradients have no graph of their own (no double backward).
 ``torch.jit.trace`` records the operators for whole sequences as calls; the steps refuse to be traced.  ``torch.compile`` leaves all
 of them out of its graphs.
 """
