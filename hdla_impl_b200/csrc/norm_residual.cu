@@ -7,10 +7,10 @@
 // row's tensors before the sums of this one; the weights wait in shared memory, so that two (backward) or four (forward) blocks
 // of 256 threads fit on an SM: with them in registers backward had one, and took 686 instead of 319 us for 32768 rows of 2048.
 // Backward computes r again from the inputs in fp32 (as many bytes as reading the rounded r), reads the norms' factors that
-// forward left (305 -> 276 us when that was done: a sum and a barrier less), takes the two sums that remain (the dot products of the norms'
-// gradients; the row that such a product belongs to is normed before the two meet, since the cube of a norm's factor need not be
-// an fp32 number where the gradient is one, as for rows of 1e12 or of 1e-14), and keeps the sums over rows (gradients of the
-// weights and of scale) in registers until its last row; blocks' sums are added in a fixed order.  Rows of more than 4096
+// forward left (305 -> 276 us when that was done: a sum and a barrier less), takes the two sums that remain (the dot products of
+// the norms' gradients), and keeps the sums over rows (gradients of the weights and of scale) in registers until its last row;
+// blocks' sums are added in a fixed order.  The row that a dot product belongs to is normed before the two meet: the cube of a
+// norm's factor need not be an fp32 number where the gradient is one, as for rows of 1e12 or of 1e-14.  Rows of more than 4096
 // channels need 1024 threads of 64 registers: there those sums are in shared memory too, and nothing is requested ahead.
 // 32768 rows of 2048, bf16, all parts: forward 139 us = 4.8 TB/s (0.75 of the measured copy), backward 269 us = 4.0 TB/s
 // (0.62); what backward waits for is the chain of its two sums.

@@ -199,7 +199,8 @@ def short_convolution(
 ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """Depthwise causal convolution: ``y_t = act(bias + sum_{k<W} weight[:, W-1-k] x_{t-k})`` for W of 1 to 8 taps.  The rows
     before a sequence come from ``initial_state`` (its last row the most recent) or are zero; the final state is the last W-1 rows
-    of (initial state, x).  Weight and bias may be of other types than x; each is used as it is, in fp32 arithmetic.  With ``cu_seqlens`` B is 1 and n the number of sequences; rows behind the last offset give zeros."""
+    of (initial state, x).  Weight and bias may be of other types than x and than each other; all arithmetic is fp32.  With
+    ``cu_seqlens`` B is 1 and n the number of sequences; rows behind the last offset give zeros."""
     if _compiling():
         return _short_convolution(x, weight, bias, activation, initial_state, output_final_state, cu_seqlens)
     silu = _silu(activation)
@@ -255,8 +256,9 @@ def selective_scan(
     x, dt, z, B, C are fp32 or bf16, all of one type; A, D, dt_bias and the states are used in fp32, and all arithmetic is fp32.
     The final state is fp32.  A call that needs gradients keeps its states at every eighth token for backward, in fp32: N / 2 bytes a
     token and channel (N rounded up to 8, 16, 32, 64 or 128; at 16 states four times x in bf16).  With HDLA_RECOMPUTE=1 in the
-    environment nothing of them is kept, and backward runs the forward pass once more.  Rows of sequences are expected to be finite (an infinite input gives NaN where the formula might
-    give an infinity).  With ``cu_seqlens`` B is 1 and n the number of sequences; rows behind the last offset give zeros."""
+    environment nothing of them is kept, and backward runs the forward pass once more.  Rows of sequences are expected to be finite
+    (an infinite input gives NaN where the formula might give an infinity).  With ``cu_seqlens`` B is 1 and n the number of
+    sequences; rows behind the last offset give zeros."""
     if _compiling():
         return _selective_scan(x, dt, A, B, C, D, z, dt_bias, dt_softplus, initial_state, output_final_state, cu_seqlens)
     cu = _offsets(cu_seqlens, x)
